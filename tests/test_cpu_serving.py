@@ -1,0 +1,144 @@
+"""Operators for several continuations of one prompt: their reference semantics, and what they refuse, without a GPU."""
+import pytest
+import torch
+
+from serving_cases import counts_of, draft_batch, page_state, prefix_batch
+from triton_distributed_b200 import ops, ref
+from triton_distributed_b200.models import PagePool
+
+
+def test_shared_prefix_reference_is_paged_attention():
+    c = prefix_batch(3, 1, 4, 2, 64, 16, 37, 20, dtype=torch.float32)
+    out, lse = ref.shared_prefix_attention_ref(**c)
+    want, want_lse = ref.paged_decode_attention_ref(c["q"], c["k_cache"], c["v_cache"], c["kv_lens"], c["block_table"], c["scale"])
+    torch.testing.assert_close(out.float(), want, rtol=1e-5, atol=1e-5)
+    torch.testing.assert_close(lse.float(), want_lse, rtol=1e-5, atol=1e-5)
+
+
+def test_verify_reference_follows_the_target():
+    """Over many draws the first token is distributed as the target says (5 tokens, 20000 draws: a frequency is off by more than
+    4.5 standard deviations, 4.5 * sqrt(0.25 / 20000) = 0.016, once in about 1e5 runs; the seed is fixed)."""
+    B, V = 20000, 5
+    g = torch.Generator().manual_seed(3)
+    p, q = torch.softmax(torch.randn(2, V, generator=g) * 1.5, -1), torch.softmax(torch.randn(1, V, generator=g) * 1.5, -1)
+    drafts = torch.multinomial(q.expand(B, V), 1, generator=g)
+    u = torch.rand(B, 2, generator=g)
+    acc, tokens = ref.verify_drafts_ref(drafts, p.expand(B, 2, V), u, q.expand(B, 1, V))
+    freq = torch.bincount(tokens[:, 0], minlength=V) / B
+    assert (freq - p[0]).abs().max() < 0.016
+    assert 0 < int(acc.sum()) < B
+
+
+@pytest.mark.parametrize("seed", range(6))
+def test_page_references_keep_the_counts(seed):
+    R, W, N, page = 9, 5, 40, 4
+    table, lens, refs = page_state(R, W, N, page, seed)
+    assert torch.equal(counts_of(table, N), refs)
+    g = torch.Generator().manual_seed(seed)
+    src, dst = torch.randint(0, R, (4,), generator=g), torch.randperm(R, generator=g)[:4]
+    table, lens, refs = ref.fork_pages_ref(table, lens, refs, src, dst, page)
+    assert torch.equal(counts_of(table, N), refs)
+    status, table, refs, copies = ref.reserve_pages_ref(table, lens, refs, (torch.rand(R, generator=g) * 4).int(), page)
+    assert torch.equal(counts_of(table, N), refs)
+    table, lens, refs = ref.trim_pages_ref(table, lens, refs, page, lens - 2)
+    assert torch.equal(counts_of(table, N), refs)
+    table, refs, moves = ref.compact_pages_ref(table, refs)
+    assert torch.equal(counts_of(table, N), refs)
+    live = int((refs > 0).sum())
+    assert bool((refs[:live] > 0).all())
+
+
+def _refused(error, call, *a, **kw):
+    with pytest.raises(error):
+        call(*a, **kw)
+
+
+def test_shared_prefix_attention_refuses():
+    ok = prefix_batch(2, 2, 4, 2, 64, 16, 32, 16)
+    call = lambda **kw: ops.shared_prefix_attention(**{**ok, **kw})  # noqa: E731
+    _refused(TypeError, call, q=ok["q"].float())
+    _refused(TypeError, call, v_cache=ok["v_cache"].to(torch.float16))
+    _refused(TypeError, call, kv_lens=ok["kv_lens"].long())
+    _refused(TypeError, call, block_table=ok["block_table"].long())
+    _refused(ValueError, call, tokens=3)
+    _refused(ValueError, call, tokens=0)
+    _refused(ValueError, call, shared=-1)
+    _refused(ValueError, call, shared=49)                                  # the table has three pages
+    _refused(ValueError, call, q=ok["q"][:, :3])                           # three query heads for two of the cache
+    _refused(ValueError, call, q=ok["q"][..., :32])
+    _refused(ValueError, call, q=ok["q"].transpose(0, 1))
+    _refused(ValueError, call, kv_lens=ok["kv_lens"][:1])
+    _refused(ValueError, call, k_cache=ok["k_cache"][:, ::2], v_cache=ok["v_cache"][:, ::2])
+    _refused(ValueError, call, prefix_table=ok["block_table"][0, :1])      # two pages are shared
+    _refused(TypeError, call, prefix_table=ok["block_table"][0].long())
+    _refused(ValueError, call, out=torch.empty(4, 4, 64))
+    wide = prefix_batch(2, 1, 4, 2, 96, 16, 32, 16)
+    _refused(ValueError, ops.shared_prefix_attention, **wide)
+    if not torch.cuda.is_available():
+        _refused(RuntimeError, call)
+    else:
+        _refused(ValueError, call)   # tensors of the CPU
+
+
+def test_verify_drafts_refuses():
+    ok = draft_batch(2, 3, 11)
+    call = lambda **kw: ops.verify_drafts(**{**ok, **kw})  # noqa: E731
+    _refused(ValueError, call, drafts=ok["drafts"][:, :2])
+    _refused(TypeError, call, drafts=ok["drafts"].int())
+    _refused(TypeError, call, uniform=ok["uniform"].double())
+    _refused(ValueError, call, uniform=ok["uniform"][:, :3])
+    _refused(TypeError, call, draft_probs=ok["draft_probs"].bfloat16())
+    _refused(TypeError, call, target_probs=ok["target_probs"].double(), draft_probs=None)
+    _refused(ValueError, call, draft_probs=ok["draft_probs"][:, :, :10])
+    _refused(TypeError, call, draft_lens=torch.tensor([1, 2]))
+    _refused(ValueError, call, draft_lens=torch.tensor([1], dtype=torch.int32))
+    _refused(ValueError, call, target_probs=ok["target_probs"].transpose(1, 2).contiguous().transpose(1, 2))
+    _refused(ValueError if torch.cuda.is_available() else RuntimeError, call)
+
+
+def test_page_operators_refuse():
+    table, lens, refs = page_state(6, 4, 30, 8)
+    caches = [torch.zeros(2, 30, 8, 4), torch.zeros(2, 30, 8, 2)]
+    here = ValueError if torch.cuda.is_available() else RuntimeError   # tensors of the CPU, or no GPU
+    _refused(TypeError, ops.fork_pages, table.long(), lens, refs, [0], [1], 8)
+    _refused(TypeError, ops.fork_pages, table[:, ::2], lens, refs, [0], [1], 8)
+    _refused(ValueError, ops.fork_pages, table, lens[:3], refs, [0], [1], 8)
+    _refused(ValueError, ops.fork_pages, table, lens, refs, [0, 1], [1], 8)
+    _refused(ValueError, ops.fork_pages, table, lens, refs, [[0]], [[1]], 8)
+    _refused(ValueError, ops.fork_pages, table, lens, refs, torch.tensor([0.0]), [1], 8)
+    _refused(ValueError, ops.fork_pages, table, lens, refs, [0], [1], 0)
+    _refused(here, ops.fork_pages, table, lens, refs, [0], [1], 8)
+    _refused(ValueError, ops.trim_pages, table, lens, refs, 8, lens[:2])
+    _refused(ValueError, ops.trim_pages, table, lens, refs, 8, lens.long())
+    _refused(here, ops.trim_pages, table, lens, refs, 8, lens)
+    _refused(ValueError, ops.reserve_pages, table, lens, refs, -1, caches, dim=1)
+    _refused(ValueError, ops.reserve_pages, table, lens, refs, lens.long(), caches, dim=1)
+    _refused(ValueError, ops.reserve_pages, table, lens, refs, 1, [], dim=1)
+    _refused(ValueError, ops.reserve_pages, table, lens, refs, 1, caches, dim=2)
+    _refused(ValueError, ops.reserve_pages, table, lens, refs, 1, caches, dim=0)                                # two pages for 30 counts
+    _refused(ValueError, ops.reserve_pages, table, lens, refs, 1, [caches[0], torch.zeros(2, 30, 4, 4)], dim=1)  # pages of other sizes
+    _refused(ValueError, ops.reserve_pages, table, lens, refs, 1, [torch.zeros(2, 30, 8, 8)[..., ::2]], dim=1)
+    _refused(here, ops.reserve_pages, table, lens, refs, 1, caches, dim=1)
+    _refused(ValueError, ops.compact_pages, table, refs, caches, dim=1, out=(table[:2], refs))
+    _refused(here, ops.compact_pages, table, refs, caches, dim=1)
+    _refused(ValueError, ops.copy_pages, caches, [0, 1], [2], dim=1)
+    _refused(ValueError, ops.copy_pages, caches, [0, 1], [2, 2], dim=1)
+    _refused(ValueError, ops.copy_pages, caches, [0, 1], [1, 2], dim=1)
+    _refused(ValueError, ops.copy_pages, caches, [0], [30], dim=1)
+    _refused(ValueError, ops.copy_pages, caches, [-1], [3], dim=1)
+    _refused(ValueError, ops.copy_pages, caches, [0], [3], dim=1, tokens=[9])
+    _refused(here, ops.copy_pages, caches, [0], [3], dim=1)
+
+
+def test_pool_slots():
+    pool = PagePool(1, 8, 3, 64, 1, 8, torch.float32, page_size=16, device="cpu")
+    pool.block_table[0, :2] = torch.tensor([3, 5])
+    pool.kv_lens[:] = torch.tensor([15, 0, 64])
+    spare = 8 * 16
+    assert pool.slots(3).tolist() == [3 * 16 + 15, 5 * 16, 5 * 16 + 1, spare, spare + 1, spare + 2, spare, spare + 1, spare + 2]
+
+
+@pytest.mark.parametrize("B,T,heads,kv,shared,own", [(1, 1, 8, 8, 0, 1), (256, 1, 8, 1, 131072, 256), (64, 1, 64, 8, 32768, 1024), (3, 8, 28, 4, 100, 50)])
+def test_prefix_splits_cover_the_keys(B, T, heads, kv, shared, own):
+    prefix, mine = ops.choose_prefix_splits(B, T, heads, kv, shared, own)
+    assert (prefix == 0) == (shared == 0) and 1 <= mine <= 64 and prefix <= 64

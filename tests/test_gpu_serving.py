@@ -1,0 +1,460 @@
+"""Operators for several continuations of one prompt against plain implementations in 64 bits."""
+import pytest
+import torch
+
+from serving_cases import counts_of, draft_batch, page_state, prefix_batch
+
+pytestmark = pytest.mark.gpu
+
+
+def _check_attention(c, out, lse, want, want_lse, spread):
+    """`spread`: sum_j w_j |v_j| of every output. The weights are rounded once to the type (half a step, u), their sum is not, the output is rounded
+    once: |error| <= u (spread + |out|). Everything else is fp32: products of at most 128 terms of scores below 40 are off by at most
+    128 * 2^-24 * 40 / 2 = 1.5e-4, which moves a weight and the log-sum-exp by that much; sums and merges add a few 2^-24 times the number of terms."""
+    u = torch.finfo(c["q"].dtype).eps / 2
+    bound = u * (spread + want.abs()) + 4e-4 * spread + 1e-6
+    off = (out.double() - want).abs()
+    assert bool((off <= bound).all()), f"{float((off / bound).max()):.2f} of the bound"
+    empty = want_lse == float("-inf")
+    assert torch.equal(lse == float("-inf"), empty)
+    assert bool((out[empty] == 0).all())
+    assert bool(((lse.double() - want_lse)[~empty].abs() <= 3e-4).all())
+
+
+def _attention_case(c, **kw):
+    from triton_distributed_b200 import ops, ref
+    want, want_lse = ref.shared_prefix_attention_ref(**c)
+    v = c["v_cache"].abs()
+    spread, _ = ref.shared_prefix_attention_ref(**{**c, "v_cache": v})
+    out, lse = ops.shared_prefix_attention(**c, return_lse=True, **kw)
+    ops.check_pipeline_status()
+    _check_attention(c, out, lse, want, want_lse, spread)
+    return out
+
+
+@pytest.mark.parametrize("B,T,Hq,Hkv,D,page,shared,own", [
+    (1, 1, 1, 1, 64, 16, 1, 1),          # one key of each
+    (1, 1, 8, 8, 128, 64, 0, 1),         # nothing shared, one key
+    (2, 1, 8, 2, 128, 64, 64, 1),
+    (3, 1, 32, 8, 128, 16, 100, 30),     # a page that ends inside a tile
+    (5, 3, 14, 2, 64, 32, 777, 90),      # groups of seven, several tokens
+    (4, 8, 28, 4, 128, 48, 1000, 61),    # pages that no tile is a multiple of
+    (2, 1, 16, 16, 64, 7, 130, 20),      # pages smaller than a slice
+    (33, 1, 8, 1, 128, 128, 3000, 200),
+    (70, 1, 40, 8, 128, 64, 513, 5),
+    (17, 5, 64, 8, 128, 256, 2048, 300),
+    (130, 2, 5, 1, 64, 64, 4100, 17),
+    (9, 1, 64, 1, 128, 16, 1500, 40),    # 64 heads on one KV head
+])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_shared_prefix_attention(B, T, Hq, Hkv, D, page, shared, own, dtype):
+    _attention_case(prefix_batch(B, T, Hq, Hkv, D, page, shared, own, dtype, seed=B + shared, device="cuda"))
+
+
+@pytest.mark.parametrize("T,shared", [(1, 200), (4, 200), (3, 64)])
+@pytest.mark.parametrize("B", [6, 150])
+def test_shared_prefix_attention_of_short_rows(T, shared, B):
+    """Rows of the batch without a sequence, sequences shorter than the shared keys, fewer keys than new tokens."""
+    lens = [shared + 9, 0, shared - 1, T - 1, shared + T - 1, 5] + [shared + i % 9 for i in range(6, B)]
+    c = prefix_batch(B, T, 16, 2, 128, 16, shared, 9, lens=lens, device="cuda")
+    _attention_case(c)
+
+
+def test_shared_prefix_attention_of_an_own_table_and_strided_rows():
+    c = prefix_batch(4, 2, 8, 2, 128, 32, 320, 40, device="cuda")
+    plain = _attention_case(c)
+    table = c["block_table"][0, :10].clone()
+    c["block_table"][:, :10] = 10 ** 6       # nobody's table is read for the shared keys
+    from triton_distributed_b200 import ops
+    torch.testing.assert_close(ops.shared_prefix_attention(**c, prefix_table=table), plain, rtol=0, atol=0)
+    wide = torch.randn(8, 12, 128, device="cuda", dtype=torch.bfloat16)   # q as columns of a wider product
+    wide[:, :8] = c["q"]
+    out = torch.full_like(c["q"], float("nan"))
+    got = ops.shared_prefix_attention(**{**c, "q": wide[:, :8]}, prefix_table=table, out=out, max_kv_len=360)
+    assert got is out
+    wide_table = torch.cat([c["block_table"], c["block_table"]], 1)[:, :c["block_table"].shape[1]]   # rows further apart than they are long
+    torch.testing.assert_close(ops.shared_prefix_attention(**{**c, "block_table": wide_table}, prefix_table=table, max_kv_len=360), out, rtol=0, atol=0)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), -float("inf")])
+def test_what_a_later_draft_holds_stays_there(dtype, bad):
+    """Values (and keys) of a drafted token that are not finite reach the tokens that see it, and no others."""
+    c = prefix_batch(3, 4, 8, 2, 128, 16, 50, 14, dtype, lens=[60, 64, 55], device="cuda")
+    from triton_distributed_b200 import ops
+    clean = ops.shared_prefix_attention(**c).view(3, 4, 8, 128)
+    page = c["block_table"][1, 62 // 16].long()     # the third of the second sequence's four tokens
+    c["v_cache"][page, 62 % 16, 1, 17] = bad
+    out = ops.shared_prefix_attention(**c).view(3, 4, 8, 128)
+    hit = torch.zeros_like(clean, dtype=torch.bool)
+    hit[1, 2:, 4:, 17] = True
+    assert torch.equal(out[~hit], clean[~hit])
+    assert not bool(out[hit].isfinite().any())
+
+
+def test_pages_outside_the_cache_count_as_zeros():
+    c = prefix_batch(3, 1, 8, 2, 64, 16, 70, 30, lens=[100, 96, 95], device="cuda")
+    c["block_table"][1, 5] = c["k_cache"].shape[0] + 5
+    c["block_table"][2, 5] = -7
+    _attention_case(c)
+
+
+def test_shared_prefix_attention_offsets_beyond_32_bits():
+    """Pages whose elements lie behind 2^31: a cache of 4.6 GB for keys and values each (only the pages in use are looked at)."""
+    N, page, Hkv, D = 140000, 128, 1, 128
+    k = torch.empty(N, page, Hkv, D, device="cuda", dtype=torch.bfloat16)
+    v = torch.empty_like(k)
+    small = prefix_batch(3, 1, 8, 1, 128, 128, 300, 100, device="cuda")
+    n = small["k_cache"].shape[0]
+    k[-n:], v[-n:] = small["k_cache"], small["v_cache"]
+    from triton_distributed_b200 import ops
+    want = ops.shared_prefix_attention(**small)
+    got = ops.shared_prefix_attention(**{**small, "k_cache": k, "v_cache": v, "block_table": small["block_table"] + (N - n)})
+    assert torch.equal(got, want)
+
+
+def _same(got, want):
+    for a, b in zip(got, want):
+        assert torch.equal(a.cpu(), b.cpu()), (a, b)
+
+
+@pytest.mark.parametrize("B,K,V", [(1, 1, 1), (1, 4, 7), (3, 0, 100), (2, 40, 33), (5, 3, 32003), (40, 2, 1001), (160, 1, 300), (2, 5, 151936)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("sampled,ragged", [(True, False), (False, True)])
+def test_verify_drafts(B, K, V, dtype, sampled, ragged):
+    from triton_distributed_b200 import ops, ref
+    c = draft_batch(B, K, V, dtype, sampled, seed=V + K, ragged=ragged)
+    _same(ops.verify_drafts(**{k: None if t is None else t.cuda() for k, t in c.items()}), ref.verify_drafts_ref(**c))
+
+
+def test_verify_drafts_edges():
+    """Numbers zero and next to one, drafts outside the vocabulary, rows without a weight, values that are no probabilities, a target equal to the
+    draft, one certain token."""
+    from triton_distributed_b200 import ops, ref
+    B, K, V = 12, 3, 5000
+    c = draft_batch(B, K, V, seed=5)
+    below_one = 1 - 2.0 ** -24
+    c["uniform"][0], c["uniform"][1] = 0.0, below_one
+    c["drafts"][2, 1], c["drafts"][3, 0] = V, -1
+    c["target_probs"][4] = 0
+    c["target_probs"][5, :, ::2] = float("nan")
+    c["draft_probs"][5, :, ::3] = float("inf")
+    c["target_probs"][6, :, 7], c["target_probs"][6, :, 11] = -1.0, float("inf")
+    c["draft_probs"][7] = c["target_probs"][7, :K]
+    c["target_probs"][8] = 0
+    c["target_probs"][8, :, 4999] = 1
+    c["drafts"][8] = 4999
+    c["draft_probs"][9] = 1.0                       # above the target everywhere: nothing is left at the refused place
+    c["uniform"][9, :K], c["uniform"][9, K] = below_one, 0.0
+    c["target_probs"][10] = 2.0 ** -149             # the smallest number of 32 bits
+    c["uniform"][11, K] = 1.0                       # not below one: the last token with a weight
+    for probs in (c["draft_probs"], None):
+        c["draft_probs"] = probs
+        want = ref.verify_drafts_ref(**c)
+        _same(ops.verify_drafts(**{k: None if t is None else t.cuda() for k, t in c.items()}), want)
+        assert int(want[1][4, 0]) == -1
+
+
+def test_verify_drafts_strided():
+    from triton_distributed_b200 import ops, ref
+    c = draft_batch(6, 3, 999, seed=9)
+    want = ref.verify_drafts_ref(**c)
+    g = {k: None if t is None else t.cuda() for k, t in c.items()}
+    wide = torch.full((4, 6, 1003), float("nan"), device="cuda")       # places first, rows longer than the vocabulary
+    wide[:, :, 1:1000] = g["target_probs"].transpose(0, 1)
+    g["target_probs"] = wide[:, :, 1:1000].transpose(0, 1)
+    g["draft_probs"] = g["draft_probs"].transpose(0, 1).contiguous().transpose(0, 1)
+    _same(ops.verify_drafts(**g), want)
+    g["draft_probs"] = g["draft_probs"][:1, :1].expand(6, 3, 999)      # one distribution for all
+    c["draft_probs"] = c["draft_probs"][:1, :1].expand(6, 3, 999)
+    _same(ops.verify_drafts(**g), ref.verify_drafts_ref(**c))
+
+
+PAGES = [(1, 1, 2, 1), (9, 5, 60, 4), (40, 12, 300, 16), (300, 6, 2500, 8), (1500, 3, 70000, 16)]
+
+
+def _caches(layers, N, page, dtype, seed=0):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    return [torch.randn(layers, N, page, 2, 24, device="cuda", generator=g).to(dtype), torch.randn(layers, N, page, 5, device="cuda", generator=g).to(dtype)]
+
+
+@pytest.mark.parametrize("R,W,N,page", PAGES)
+@pytest.mark.parametrize("seed", [0, 1])
+def test_fork_and_trim_pages(R, W, N, page, seed):
+    from triton_distributed_b200 import ops, ref
+    table, lens, refs = page_state(R, W, N, page, seed)
+    g = torch.Generator().manual_seed(seed)
+    n = max(1, R // 2)
+    src, dst = torch.randint(-1, R + 1, (n,), generator=g), torch.randint(-1, R + 1, (n,), generator=g)   # some out of range, some named twice
+    want = ref.fork_pages_ref(table, lens, refs, src, dst, page)
+    got = [t.cuda() for t in (table, lens, refs)]
+    ops.fork_pages(*got, src.cuda() if seed else src.tolist(), dst.int().cuda(), page)
+    _same(got, want)
+    cut = torch.randint(-2, W * page + 2, (R,), generator=g, dtype=torch.int32)
+    want = ref.trim_pages_ref(*want, page, cut)
+    ops.trim_pages(*got, page, cut.cuda())
+    _same(got, want)
+    rows = [0, R - 1, 0, R, -1]
+    want = ref.trim_pages_ref(*want, page, None, rows)
+    ops.trim_pages(*got, page, None, rows)
+    _same(got, want)
+    assert torch.equal(counts_of(got[0].cpu(), N), got[2].cpu())
+
+
+def test_fork_exchanges_rows():
+    from triton_distributed_b200 import ops
+    table, lens, refs = (t.cuda() for t in page_state(9, 5, 60, 4, 3))
+    old = table.clone(), lens.clone(), refs.clone()
+    ops.trim_pages(table, lens, refs, 4, lens.clone())     # room behind the last token is not forked
+    trimmed = table.clone()
+    ops.fork_pages(table, lens, refs, list(range(9)), list(range(8, -1, -1)), 4)
+    assert torch.equal(table, trimmed.flip(0)) and torch.equal(lens, old[1].flip(0))
+    ops.fork_pages(table, lens, refs, [], [], 4)
+
+
+@pytest.mark.parametrize("R,W,N,page", PAGES)
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32, torch.uint8])
+def test_reserve_pages(R, W, N, page, dtype):
+    from triton_distributed_b200 import ops, ref
+    table, lens, refs = page_state(R, W, N, page, 1)
+    lens = torch.minimum(lens, torch.full_like(lens, W * page - 3)).clamp_min(0)   # room in the table for all
+    table, lens, refs = ref.trim_pages_ref(table, lens, refs, page, lens) if R < 1000 else (table, lens, refs)
+    g = torch.Generator().manual_seed(2)
+    src, dst = torch.randint(0, R, (R // 2,), generator=g), torch.randperm(R, generator=g)[:R // 2]
+    table, lens, refs = ref.fork_pages_ref(table, lens, refs, src, dst, page)
+    counts = torch.randint(0, 4, (R,), generator=g, dtype=torch.int32)
+    caches = _caches(2, N if N < 5000 else 3000, page, dtype) if N < 5000 else None
+    if caches is None:   # the tables alone are large
+        caches = [torch.zeros(N, page, 1, device="cuda", dtype=torch.uint8)]
+    dim = 0 if N >= 5000 else 1
+    before = [t.clone() for t in caches]
+    for count in (counts, 2):
+        status, want_table, want_refs, copies = ref.reserve_pages_ref(table, lens, refs, count, page)
+        got = [t.cuda() for t in (table, lens, refs)]
+        now = [t.clone() for t in before]
+        st = ops.reserve_pages(*got, count.cuda() if isinstance(count, torch.Tensor) else count, now, dim=dim)
+        assert int(st) == status
+        _same(got, (want_table, lens, want_refs))
+        for t, old in zip(now, before):
+            want = old.clone()
+            for a, b, n in copies:
+                want.select(dim, b).narrow(dim, 0, n).copy_(old.select(dim, a).narrow(dim, 0, n))
+            assert torch.equal(t, want)
+
+
+def test_reserve_pages_without_pages():
+    from triton_distributed_b200 import ops
+    caches = [torch.arange(6 * 4, device="cuda", dtype=torch.float32).view(6, 4, 1)]
+    table = torch.tensor([[0, 1, -1], [0, 1, -1], [2, -1, -1]], dtype=torch.int32, device="cuda")
+    lens = torch.tensor([6, 6, 4], dtype=torch.int32, device="cuda")
+    refs = torch.tensor([2, 2, 1, 1, 1, 0], dtype=torch.int32, device="cuda")   # one page is free: two are needed
+    state = [t.clone() for t in (table, lens, refs, caches[0])]
+    assert int(ops.reserve_pages(table, lens, refs, 1, caches)) == 1
+    assert all(torch.equal(a, b) for a, b in zip((table, lens, refs, caches[0]), state))
+    assert int(ops.reserve_pages(table, lens, refs, 9, caches)) == 2            # longer than a row of the table
+    assert all(torch.equal(a, b) for a, b in zip((table, lens, refs, caches[0]), state))
+    one = torch.tensor([1, 1, 0], dtype=torch.int32, device="cuda")
+    assert int(ops.reserve_pages(table, lens, refs, one, caches)) == 0          # one copy is enough: the first row keeps the page
+    assert table.tolist() == [[0, 1, -1], [0, 5, -1], [2, -1, -1]] and refs.tolist() == [2, 1, 1, 1, 1, 1]
+    assert caches[0][5].flatten().tolist() == [4.0, 5.0, 22.0, 23.0]
+    assert int(ops.reserve_pages(table, lens, refs, torch.zeros_like(one), caches)) == 0
+
+
+@pytest.mark.parametrize("R,W,N,page", PAGES)
+@pytest.mark.parametrize("inplace", [True, False])
+def test_compact_pages(R, W, N, page, inplace):
+    from triton_distributed_b200 import ops, ref
+    table, lens, refs = page_state(R, W, N, page, 4)
+    want_table, want_refs, moves = ref.compact_pages_ref(table, refs)
+    caches = _caches(3, N, page, torch.float16) if N < 5000 else [torch.randint(0, 255, (1, N, page, 3), device="cuda", dtype=torch.uint8)]
+    before = [t.clone() for t in caches]
+    a, b = table.cuda(), refs.cuda()
+    got = ops.compact_pages(a, b, caches, dim=1, out=(a, b) if inplace else None)
+    _same(got, (want_table, want_refs))
+    if not inplace:
+        _same((a, b), (table, refs))
+    if moves:
+        src, dst = (torch.tensor(x, device="cuda") for x in zip(*moves))
+        for t in before:
+            t[:, dst] = t[:, src]
+    for t, old in zip(caches, before):
+        assert torch.equal(t, old)
+
+
+@pytest.mark.parametrize("shape,dim,dtype", [((20, 4, 3), 0, torch.uint8), ((20, 7, 5), 0, torch.bfloat16), ((3, 20, 16, 2, 64), 1, torch.float16),
+                                             ((2, 20, 64, 8, 128), 1, torch.bfloat16), ((20, 3, 2), 0, torch.float64)])
+def test_copy_pages(shape, dim, dtype):
+    from triton_distributed_b200 import ops
+    many = [(torch.rand(shape, device="cuda") * 200).to(dtype) for _ in range(60 if len(shape) == 3 else 2)]   # more tensors than a launch takes
+    before = [t.clone() for t in many]
+    src, dst, n = [3, 3, 19, 0], [1, 2, 4, 7], [shape[dim + 1], 1, 0, 2]
+    ops.copy_pages(many, src, dst, dim, n)
+    for t, old in zip(many, before):
+        for a, b, k in zip(src, dst, n):
+            old.select(dim, b).narrow(dim, 0, k).copy_(old.select(dim, a).narrow(dim, 0, k))
+        assert torch.equal(t, old)
+    ops.copy_pages(many, [3], [1], dim)
+    assert torch.equal(many[0].select(dim, 1), many[0].select(dim, 3))
+    ops.copy_pages(many, [], [], dim)
+
+
+def _write(pool, layer, slots, k, v):
+    pool.layer(layer)[0].view(-1, pool.kv_heads, pool.head_dim)[slots] = k
+    pool.layer(layer)[1].view(-1, pool.kv_heads, pool.head_dim)[slots] = v
+
+
+def test_a_prompt_continued_by_drafts():
+    """The operators as they are used together: a prompt is prefilled once and forked, all rows draft, write, attend and are cut back to what was accepted;
+    rows end, the cache is compacted, the rest goes on. Attention is that of every row's own text, kept apart on the side."""
+    from triton_distributed_b200 import ops
+    from triton_distributed_b200.models import PagePool
+    torch.manual_seed(0)
+    R, K, Hkv, Hq, D, page, V = 6, 3, 2, 8, 128, 16, 700
+    pool = PagePool(2, 70, R, 400, Hkv, D, page_size=page)
+    text = [[None, None] for _ in range(R)]        # per row and layer: keys and values of its tokens
+    prompt = 75
+    count = torch.zeros(R, dtype=torch.int32, device="cuda")
+    count[0] = prompt
+    pool.reserve(count)
+    slots = pool.slots(prompt)[:prompt]
+    for i in range(2):
+        kv = torch.randn(2, prompt, Hkv, D, device="cuda", dtype=torch.bfloat16)
+        _write(pool, i, slots, *kv)
+        text[0][i] = kv
+    pool.advance(count)
+    live = list(range(R))
+    pool.fork([0] * (R - 1), list(range(1, R)))
+    for r in range(1, R):
+        text[r] = list(text[0])
+    assert int((pool.refs > 0).sum()) == 5         # one copy of the prompt
+    T = K + 1
+    for step in range(12):
+        active = torch.zeros(R, dtype=torch.int32, device="cuda")
+        active[live] = T
+        start = pool.kv_lens.clone()
+        pool.reserve(active)
+        slots = pool.slots(T)
+        pool.advance(active)
+        for i in range(2):
+            new = torch.randn(2, R, T, Hkv, D, device="cuda", dtype=torch.bfloat16)
+            _write(pool, i, slots, *new.view(2, R * T, Hkv, D))
+            q = torch.randn(R * T, Hq, D, device="cuda", dtype=torch.bfloat16)
+            first = pool.block_table[live[0]].contiguous()
+            out = ops.shared_prefix_attention(q, *pool.layer(i), pool.kv_lens, pool.block_table, prompt, D ** -0.5, tokens=T, prefix_table=first)
+            for r in range(R):
+                if r not in live:
+                    assert bool((out[r * T:(r + 1) * T] == 0).all())
+                    continue
+                text[r][i] = torch.cat([text[r][i], new[:, r]], 1)
+                k, v = text[r][i].float()
+                n = k.shape[0]
+                s = torch.einsum("tkgd,nkd->tkgn", q[r * T:(r + 1) * T].float().view(T, Hkv, Hq // Hkv, D), k) * D ** -0.5
+                s.masked_fill_(torch.arange(n, device="cuda") > (n - T + torch.arange(T, device="cuda"))[:, None, None, None], float("-inf"))
+                want = torch.einsum("tkgn,nkd->tkgd", s.softmax(-1), v).reshape(T, Hq, D)
+                # rounded weights and output: 2^-8 (spread + |out|) with |v| below 5.5 and the weights' sum one
+                torch.testing.assert_close(out[r * T:(r + 1) * T].float(), want, rtol=2 ** -7, atol=2 ** -6)
+        d = draft_batch(R, K, V, seed=step, device="cuda")
+        accepted, tokens = ops.verify_drafts(**d)
+        keep = start + accepted + 1                # the token before the drafts, and the drafts that stand
+        pool.trim(torch.where(active > 0, keep, -1).int())
+        for r in live:
+            text[r] = [t[:, :int(keep[r])] for t in text[r]]
+        assert torch.equal(counts_of(pool.block_table.cpu(), 70), pool.refs.cpu())
+        if step in (3, 6):
+            pool.free([live.pop(1)])
+            pool.compact()
+            n = int((pool.refs > 0).sum())
+            assert bool((pool.refs[:n] > 0).all()) and int(pool.block_table.max()) < n
+        if step == 8:                              # one of them branches again, from where it stands
+            pool.fork([live[1]], [1])
+            text[1] = list(text[live[1]])
+            live.append(1)
+    with pytest.raises(RuntimeError):
+        pool.reserve(399)
+    with pytest.raises(RuntimeError):
+        pool.reserve(torch.full((R,), 250, dtype=torch.int32, device="cuda"))
+
+
+def test_a_captured_step():
+    """A step in a graph, replayed on other data and next to a second graph and eager calls; results are those of the step alone."""
+    from triton_distributed_b200 import ops
+    from triton_distributed_b200.models import PagePool
+    R, page, K = 4, 16, 2
+
+    def make(seed):
+        torch.manual_seed(seed)
+        pool = PagePool(1, 40, R, 200, 2, 64, page_size=page)
+        pool.k_cache.normal_(), pool.v_cache.normal_()
+        n = torch.zeros(R, dtype=torch.int32, device="cuda")
+        n[0] = 70
+        pool.reserve(n), pool.advance(n)
+        pool.fork([0, 0, 0], [1, 2, 3])
+        return {"pool": pool, "q": torch.randn(R * 3, 8, 64, device="cuda", dtype=torch.bfloat16), **draft_batch(R, K, 300, seed=seed, device="cuda")}
+
+    def step(s):
+        pool = s["pool"]
+        pool.reserve(3, check=False)
+        pool.advance(3)
+        out = ops.shared_prefix_attention(s["q"], *pool.layer(0), pool.kv_lens, pool.block_table, 70, 0.125, tokens=3)
+        accepted, tokens = ops.verify_drafts(s["drafts"], s["target_probs"], s["uniform"], s["draft_probs"])
+        pool.trim(pool.kv_lens - K + accepted)
+        return out, accepted, tokens
+
+    eager, results = [make(0), make(1)], []
+    for s in eager:
+        results.append([[t.clone() for t in step(s)] + [s["pool"].kv_lens.clone(), s["pool"].block_table.clone()] for _ in range(4)])
+    states, graphs, outs = [make(0), make(1)], [], []
+    for s in states:
+        keep = [t.clone() for t in (s["pool"].block_table, s["pool"].kv_lens, s["pool"].refs)]
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            step(s)
+        torch.cuda.current_stream().wait_stream(side)
+        for t, old in zip((s["pool"].block_table, s["pool"].kv_lens, s["pool"].refs), keep):
+            t.copy_(old)
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append(step(s))
+        graphs.append(g)
+    third = make(2)
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    torch.cuda.synchronize()
+    for i in range(4):
+        for j in (0, 1):
+            with torch.cuda.stream(streams[j]):
+                graphs[j].replay()
+        if i == 0:
+            step(third)
+        torch.cuda.synchronize()
+        for j in (0, 1):
+            got = [*outs[j], states[j]["pool"].kv_lens, states[j]["pool"].block_table]
+            assert all(torch.equal(a, b) for a, b in zip(got, results[j][i])), (i, j)
+    ops.check_pipeline_status()
+
+
+def test_two_calls_on_two_streams():
+    from triton_distributed_b200 import ops
+    cases = [prefix_batch(40, 1, 32, 8, 128, 64, 3000, 100, seed=s, device="cuda") for s in (0, 1)]
+    want = [ops.shared_prefix_attention(**c) for c in cases]
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(10):
+        for j in (0, 1):
+            with torch.cuda.stream(streams[j]):
+                got[j].append(ops.shared_prefix_attention(**cases[j]))
+    torch.cuda.synchronize()
+    for j in (0, 1):
+        assert all(torch.equal(g, want[j]) for g in got[j])
+
+
+def test_empty_calls():
+    from triton_distributed_b200 import ops
+    k = torch.zeros(4, 16, 2, 64, device="cuda", dtype=torch.bfloat16)
+    z = lambda *s: torch.zeros(*s, dtype=torch.int32, device="cuda")  # noqa: E731
+    out = ops.shared_prefix_attention(torch.empty(0, 4, 64, device="cuda", dtype=torch.bfloat16), k, k, z(0), z(0, 3), 0, 1.0)
+    assert out.shape == (0, 4, 64)
+    c = draft_batch(0, 2, 5, sampled=False, device="cuda")
+    accepted, tokens = ops.verify_drafts(**c)
+    assert accepted.shape == (0,) and tokens.shape == (0, 3)

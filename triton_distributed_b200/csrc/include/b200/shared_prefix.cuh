@@ -1,0 +1,27 @@
+// What the kernels of the shared-prefix attention (shared_prefix.cu, shared_prefix_sm100.cu) are told.
+#pragma once
+#include <cstdint>
+
+namespace b200 {
+
+struct SharedPrefixParams {
+  const void* q;            // [B * T, Hq, D], ldq elements between tokens
+  const void* k_cache;      // [num_blocks, page, Hkv, D]
+  const void* v_cache;
+  const int* kv_lens;       // [B], the T new tokens counted
+  const int* block_table;   // [B, width], bt_stride between rows
+  const int* prefix_table;  // [>= ceil(shared / page)]
+  float* o_part;            // [B * T * Hq, S, D]
+  float* lse_part;          // [B * T * Hq, S], natural logarithm; -inf: an empty range, whose o_part is not read
+  uint32_t* status;         // nullable: set non-zero when a pipeline wait expired
+  long long ldq;
+  int bt_stride, width, B, T, Hq, Hkv, num_blocks, page;
+  int shared;               // keys that all sequences begin with
+  int prefix_splits, own_splits, S;   // ranges of keys per row: S = prefix_splits + own_splits
+  int prefix_chunk;         // keys per range of the shared ones, a multiple of 64
+  int prefix_ctas;          // CTAs of the shared keys in the span kernel's grid
+  int late_wait;            // the kernel in front is this call's own: only the end of the span kernel waits for it
+  float scale_log2e;        // softmax scale * log2(e)
+};
+
+}  // namespace b200

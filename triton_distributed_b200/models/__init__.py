@@ -2,7 +2,7 @@
 from .auto import AutoLLM, AutoTokenizer
 from .config import ARCHS, ArchConfig, LikosunConfig, ModelConfig, SizilornConfig
 from .engine import Engine
-from .kv_cache import HybridCache, KV_Cache, LatentCache
+from .kv_cache import HybridCache, KV_Cache, LatentCache, PagePool
 from .likosun import Likosun
 from .qwen import Qwen3
 from .sizilorn import Sizilorn
@@ -10,5 +10,5 @@ from .utils import logger, sample_token, seed_everything
 
 
 __all__ = ["ARCHS", "ArchConfig", "LikosunConfig", "SizilornConfig", "ModelConfig", "AutoLLM", "AutoTokenizer", "Qwen3", "Likosun",
-           "Sizilorn", "KV_Cache", "LatentCache", "HybridCache", "Engine",
+           "Sizilorn", "KV_Cache", "LatentCache", "HybridCache", "PagePool", "Engine",
            "sample_token", "seed_everything", "logger"]

@@ -14,6 +14,8 @@ import dataclasses
 
 import torch
 
+from .. import ops
+
 
 class PagedCache:
 
@@ -145,3 +147,70 @@ class HybridCache(PagedCache):
     def restore_state(self, saved) -> None:
         for t, old in zip(self._all_states(), saved):
             t.copy_(old)
+
+
+class PagePool:
+    """Keys and values of rows that may hold the same pages: several samples of a prompt, beams, drafts that are taken back.
+
+    Unlike in a ``PagedCache`` no row owns a fixed run of pages: ``block_table`` int32 [batch, max_blocks] (-1: not held), ``kv_lens`` int32 [batch] and
+    ``refs`` int32 [num_blocks] (how many rows hold a page) live on the device and are changed in place by kernels, so that a step can be
+    captured. A step of S tokens: ``reserve(S)``, keys and values to ``slots(S)``, ``advance(S)``, attention over ``layer(i)``, ``kv_lens`` and
+    ``block_table`` (``ops.decode_attention``, ``ops.shared_prefix_attention``); drafts that were refused go with ``trim``. The caches have one page
+    more than ``refs`` counts: rows without room write there."""
+
+    def __init__(self, num_layers: int, num_blocks: int, batch_size: int, max_length: int, kv_heads: int, head_dim: int = 128, dtype=torch.bfloat16,
+                 page_size: int = 64, device="cuda") -> None:
+        self.num_layers, self.num_blocks, self.batch_size, self.max_length = num_layers, num_blocks, batch_size, max_length
+        self.kv_heads, self.head_dim, self.dtype, self.page_size = kv_heads, head_dim, dtype, page_size
+        shape = (num_layers, num_blocks + 1, page_size, kv_heads, head_dim)
+        self.k_cache = torch.zeros(shape, device=device, dtype=dtype)
+        self.v_cache = torch.zeros(shape, device=device, dtype=dtype)
+        self.block_table = torch.full((batch_size, (max_length + page_size - 1) // page_size), -1, dtype=torch.int32, device=device)
+        self.kv_lens = torch.zeros(batch_size, dtype=torch.int32, device=device)
+        self.refs = torch.zeros(num_blocks, dtype=torch.int32, device=device)
+        self.status = torch.zeros(1, dtype=torch.int32, device=device)
+
+    def layer(self, layer_idx: int):
+        """(k pages, v pages) of one layer: [num_blocks + 1, page, kv_heads, head_dim]."""
+        return self.k_cache[layer_idx], self.v_cache[layer_idx]
+
+    def fork(self, src, dst) -> None:
+        """Rows `dst[i]` continue what rows `src[i]` hold (``ops.fork_pages``); no data moves."""
+        ops.fork_pages(self.block_table, self.kv_lens, self.refs, src, dst, self.page_size)
+
+    def reserve(self, count, check: bool = True) -> None:
+        """Room for `count` more tokens (a number, or int32 [batch]) in every row (``ops.reserve_pages``). ``check``: wait for the outcome and
+        raise where there are too few pages; without it (inside a capture) ``status`` tells."""
+        ops.reserve_pages(self.block_table, self.kv_lens, self.refs, count, (self.k_cache, self.v_cache), dim=1, status=self.status)
+        if check:
+            self.check()
+
+    def check(self) -> None:
+        """Raise if the last ``reserve`` found too few pages, or a row that would outgrow its table (nothing has been changed then)."""
+        code = int(self.status.item())
+        if code:
+            raise RuntimeError("PagePool: too few free pages" if code == 1 else "PagePool: a row would exceed max_length")
+
+    def slots(self, count: int) -> torch.Tensor:
+        """Flat slot (page * page_size + offset) of the next `count` tokens of every row -> int64 [batch * count]; the spare page for rows without room."""
+        pos = self.kv_lens[:, None].to(torch.int64) + torch.arange(count, device=self.kv_lens.device)[None, :]
+        at = pos // self.page_size
+        blk = self.block_table.gather(1, at.clamp_max(self.block_table.shape[1] - 1)).to(torch.int64)
+        blk = torch.where((blk >= 0) & (at < self.block_table.shape[1]), blk, self.num_blocks)
+        return (blk * self.page_size + pos % self.page_size).reshape(-1)
+
+    def advance(self, count) -> None:
+        """The next `count` tokens (a number, or int32 [batch]) of every row have been written."""
+        self.kv_lens += count
+
+    def trim(self, lens: torch.Tensor, rows=None) -> None:
+        """Rows keep their first `lens` tokens (``ops.trim_pages``)."""
+        ops.trim_pages(self.block_table, self.kv_lens, self.refs, self.page_size, lens, rows)
+
+    def free(self, rows) -> None:
+        """Rows give back all they hold."""
+        ops.trim_pages(self.block_table, self.kv_lens, self.refs, self.page_size, None, rows)
+
+    def compact(self) -> None:
+        """The pages in use move to the front of the caches (``ops.compact_pages``)."""
+        ops.compact_pages(self.block_table, self.refs, (self.k_cache, self.v_cache), dim=1, out=(self.block_table, self.refs))

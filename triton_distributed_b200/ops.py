@@ -968,3 +968,264 @@ def prefill_attention_vt(q: torch.Tensor, k: torch.Tensor, vt: torch.Tensor, cu_
               1 if causal else 0, ptr(sink), ptr(out), dtype_code(q.dtype), ptr(_pipeline_status(q.device)), stream_ptr())
     _count()
     return out
+
+
+# ---- several continuations of one prompt (csrc/kernels/shared_prefix.cu, verify.cu, pages.cu) --
+def _check_device(name: str, *tensors: torch.Tensor | None) -> None:
+    """All tensors on the current CUDA device: the kernels are launched on its current stream."""
+    _lib.require_cuda()
+    current = torch.cuda.current_device()
+    for t in tensors:
+        if t is not None and (not t.is_cuda or t.device.index != current):
+            raise ValueError(f"{name}: all tensors must be on the current CUDA device (cuda:{current}), got {t.device}")
+
+
+@functools.lru_cache(maxsize=1024)
+def choose_prefix_splits(batch: int, tokens: int, heads: int, kv_heads: int, shared: int, own: int, sm_count: int = 148) -> tuple[int, int]:
+    """Ranges of keys (of the shared keys, of everybody's own) for `shared_prefix_attention`: one wave of two CTAs per SM, all with about
+    as many keys, at least 128."""
+    group = heads // kv_heads
+    rows = batch * tokens * group
+    prefix_ctas = kv_heads * -(-rows // (32 if rows > 16 else 16)) if shared else 0
+    own_ctas = batch * kv_heads * -(-tokens * group // (32 if tokens * group > 16 else 16))
+    share = max(128, (prefix_ctas * shared + own_ctas * own) // (2 * sm_count))
+    chunk = -(-share // 64) * 64
+    return (min(64, -(-shared // chunk)) if shared else 0), max(1, min(64, -(-own // chunk)))
+
+
+def shared_prefix_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, kv_lens: torch.Tensor, block_table: torch.Tensor,
+                            shared: int, scale: float, tokens: int = 1, prefix_table: torch.Tensor | None = None, max_kv_len: int | None = None,
+                            out: torch.Tensor | None = None, return_lse: bool = False):
+    """Paged causal attention of the last `tokens` tokens of every sequence, where the first `shared` keys of all sequences are the same and
+    are read once for the whole batch: several samples of one prompt, questions about one document, drafted tokens (``tokens`` > 1).
+
+    q [B * tokens, Hq, D], 16-bit, rows may be strided; caches [num_blocks, page, Hkv, D] in the type of q, D 64 or 128; kv_lens int32 [B] with the
+    new tokens; block_table int32 [B, max_blocks]. Query token t of sequence b attends keys j < kv_lens[b] - tokens + t + 1; a row
+    without any gives zeros. Keys j < ``shared`` are read through ``prefix_table`` (int32 [>= ceil(shared / page)], default: the first
+    sequence's row of the block table) for every sequence that reaches beyond them with all its tokens; shorter sequences (also
+    kv_lens 0) are attended over their own table alone. ``shared`` need not be a multiple of the page. ``max_kv_len``: an upper bound on kv_lens for the choice
+    of splits (default: what the table can hold). Returns [B * tokens, Hq, D] (and the natural-log LSE fp32 [B * tokens, Hq])."""
+    if q.dim() != 3 or k_cache.dim() != 4 or k_cache.shape != v_cache.shape or kv_lens.dim() != 1 or block_table.dim() != 2:
+        raise ValueError("shared_prefix_attention: q [B * tokens, Hq, D], caches [num_blocks, page, Hkv, D], kv_lens [B], block_table [B, max_blocks]")
+    T, Hq, D = q.shape
+    N, page, Hkv, Dk = k_cache.shape
+    B, width = block_table.shape
+    shared, tokens = int(shared), int(tokens)
+    if q.dtype not in (torch.bfloat16, torch.float16) or k_cache.dtype != q.dtype or v_cache.dtype != q.dtype:
+        raise TypeError("shared_prefix_attention handles bf16 / f16 (q and caches of one type)")
+    if D not in (64, 128) or Dk != D:
+        raise ValueError(f"shared_prefix_attention: head sizes 64 and 128, got {D} and {Dk}")
+    if tokens < 1 or T != B * tokens or kv_lens.shape[0] != B or Hkv < 1 or Hq % Hkv or Hq < 1 or N < 1 or page < 1:
+        raise ValueError("shared_prefix_attention: the batch, token or head counts do not fit together")
+    if kv_lens.dtype != torch.int32 or block_table.dtype != torch.int32 or (prefix_table is not None and prefix_table.dtype != torch.int32):
+        raise TypeError("shared_prefix_attention: kv_lens and the tables are int32")
+    if not (k_cache.is_contiguous() and v_cache.is_contiguous() and kv_lens.is_contiguous()) or (width > 1 and block_table.stride(1) != 1):
+        raise ValueError("shared_prefix_attention needs contiguous caches and lengths and a row-major block table")
+    if q.stride(2) != 1 or (Hq > 1 and q.stride(1) != D) or (T > 1 and (q.stride(0) % 8 or q.stride(0) < 0)) or (q.data_ptr() | k_cache.data_ptr() | v_cache.data_ptr()) % 16:
+        raise ValueError("shared_prefix_attention: q holds whole rows of heads, a multiple of 8 elements apart; q and caches start on 16 bytes")
+    blocks = -(-shared // page)
+    if shared < 0 or (shared > 0 and prefix_table is None and (width < blocks or B == 0)):
+        raise ValueError(f"shared_prefix_attention: {shared} shared keys do not fit the block table")
+    if prefix_table is None:
+        prefix_table = block_table
+    elif prefix_table.dim() != 1 or prefix_table.shape[0] < blocks or not prefix_table.is_contiguous():
+        raise ValueError("shared_prefix_attention: the prefix table holds the pages of the shared keys")
+    if out is not None and (out.shape != q.shape or out.dtype != q.dtype or not out.is_contiguous()):
+        raise ValueError("shared_prefix_attention: the output is contiguous and has the shape and type of q")
+    _check_device("shared_prefix_attention", q, k_cache, v_cache, kv_lens, block_table, prefix_table, out)
+    if out is None:
+        out = torch.empty((T, Hq, D), dtype=q.dtype, device=q.device)
+    lse = torch.empty((T, Hq), dtype=torch.float32, device=q.device) if return_lse else None
+    if B:
+        longest = width * page if max_kv_len is None else min(int(max_kv_len), width * page)
+        prefix_splits, own_splits = choose_prefix_splits(B, tokens, Hq, Hkv, shared, max(1, longest - shared))
+        ranges = T * Hq * (prefix_splits + own_splits)
+        part = torch.empty(ranges * (D + 1), dtype=torch.float32, device=q.device)   # outputs of all ranges, then their log-sum-exps
+        at = part.data_ptr()
+        _lib.call("b200_shared_prefix_attention", ptr(q), ctypes.c_longlong(q.stride(0) if T > 1 else Hq * D), ptr(k_cache), ptr(v_cache), ptr(kv_lens),
+                  ptr(block_table), block_table.stride(0), width, ptr(prefix_table), B, tokens, Hq, Hkv, D, N, page, shared, c_float(scale),
+                  prefix_splits, own_splits, ctypes.c_void_p(at), ctypes.c_void_p(at + ranges * D * 4), ptr(out), ptr(lse), dtype_code(q.dtype),
+                  ptr(_pipeline_status(q.device)), stream_ptr())
+        _count(2)
+    return (out, lse) if return_lse else out
+
+
+def verify_drafts(drafts: torch.Tensor, target_probs: torch.Tensor, uniform: torch.Tensor, draft_probs: torch.Tensor | None = None,
+                  draft_lens: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+    """Which drafted tokens stand, and the token behind them, so that the tokens are distributed as if sampled from the target alone.
+
+    drafts int64 [B, K]; target_probs [B, K + 1, V] (fp32, bf16 or f16; row i: the target's probabilities at the place of draft i);
+    draft_probs [B, K, V] in the same type: what the drafts were sampled from (None: they were picked without chance); uniform fp32 [B, K + 1] in
+    [0, 1); draft_lens int32 [B]: drafts of every sequence (default K, K may be 0). Draft i is accepted if those before it are and
+    ``uniform[i] * draft_probs[i, d_i] < target_probs[i, d_i]``; the next token is drawn with ``uniform[K]`` from the positive part of target
+    minus draft at the first refused place (the target itself where nothing is left), or from the target behind the last draft. Rows need not sum to one;
+    what is not positive and finite counts as zero, drafts outside the vocabulary are refused.
+
+    Returns (accepted int32 [B], tokens int64 [B, K + 1]: the accepted drafts, the drawn token (-1 if nothing has a weight), then -1)."""
+    if drafts.dim() != 2 or target_probs.dim() != 3:
+        raise ValueError("verify_drafts: drafts [B, K], target_probs [B, K + 1, V]")
+    B, K = drafts.shape
+    V = target_probs.shape[2]
+    if target_probs.shape[:2] != (B, K + 1) or V < 1 or uniform.shape != (B, K + 1) or (draft_probs is not None and draft_probs.shape != (B, K, V)) \
+            or (draft_lens is not None and draft_lens.shape != (B,)):
+        raise ValueError("verify_drafts: target_probs [B, K + 1, V], uniform [B, K + 1], draft_probs [B, K, V], draft_lens [B]")
+    if drafts.dtype != torch.int64 or uniform.dtype != torch.float32 or (draft_lens is not None and draft_lens.dtype != torch.int32):
+        raise TypeError("verify_drafts: drafts int64, uniform fp32, draft_lens int32")
+    if target_probs.dtype not in (torch.float32, torch.bfloat16, torch.float16) or (draft_probs is not None and draft_probs.dtype != target_probs.dtype):
+        raise TypeError("verify_drafts: probabilities of one type, fp32, bf16 or f16")
+    if (V > 1 and (target_probs.stride(2) != 1 or (draft_probs is not None and K > 0 and draft_probs.stride(2) != 1))) or not drafts.is_contiguous() \
+            or not uniform.is_contiguous() or (draft_lens is not None and not draft_lens.is_contiguous()):
+        raise ValueError("verify_drafts: probabilities with unit stride along the vocabulary, the rest contiguous")
+    _check_device("verify_drafts", drafts, target_probs, uniform, draft_probs, draft_lens)
+    accepted = torch.empty(B, dtype=torch.int32, device=drafts.device)
+    tokens = torch.empty((B, K + 1), dtype=torch.int64, device=drafts.device)
+    ll = ctypes.c_longlong
+    d_b, d_k = (draft_probs.stride(0), draft_probs.stride(1)) if draft_probs is not None else (0, 0)
+    if B:
+        _lib.call("b200_verify_drafts", ptr(drafts), ptr(target_probs), ll(target_probs.stride(0)), ll(target_probs.stride(1)), ptr(draft_probs), ll(d_b),
+                  ll(d_k), ptr(uniform), ptr(draft_lens), B, K, V, ptr(accepted), ptr(tokens), dtype_code(target_probs.dtype), stream_ptr())
+        _count()
+    return accepted, tokens
+
+
+class _PageTensor(ctypes.Structure):
+    """Mirror of ``b200::PageTensor`` (csrc/kernels/pages.cu)."""
+    _fields_ = [("base", ctypes.c_void_p), ("layers", ctypes.c_longlong), ("layer_stride", ctypes.c_longlong), ("page_bytes", ctypes.c_longlong),
+                ("row_bytes", ctypes.c_longlong)]
+
+
+def _page_tensors(name: str, caches, dim: int, pages: int | None = None):
+    """(native descriptions, tokens per page) of tensors whose dimension `dim` (0, or 1 behind layers) counts pages."""
+    caches = list(caches)
+    if dim not in (0, 1):
+        raise ValueError(f"{name}: pages are counted by dimension 0, or 1 behind the layers")
+    page, out = None, (_PageTensor * max(1, len(caches)))()
+    for i, t in enumerate(caches):
+        if t.dim() < dim + 2 or (pages is not None and t.shape[dim] < pages) or t.numel() == 0:
+            raise ValueError(f"{name}: a cache is [{'layers, ' if dim else ''}pages, tokens, ...] with as many pages as the counts have")
+        if page is not None and t.shape[dim + 1] != page:
+            raise ValueError(f"{name}: the caches differ in the tokens of a page")
+        page = t.shape[dim + 1]
+        one = t[0] if dim else t
+        if not one.is_contiguous():
+            raise ValueError(f"{name}: the pages of a layer must be contiguous")
+        size, row = t.element_size(), one[0, 0].numel()
+        out[i] = _PageTensor(t.data_ptr(), t.shape[0] if dim else 1, t.stride(0) * size if dim else 0, page * row * size, row * size)
+    return caches, out, page
+
+
+def _check_page_state(name: str, block_table, refs, kv_lens=None, page=1) -> tuple[int, int, int]:
+    if block_table.dim() != 2 or refs.dim() != 1 or not block_table.numel() or not refs.numel() or (kv_lens is not None and kv_lens.shape != block_table.shape[:1]):
+        raise ValueError(f"{name}: block_table [rows, max_blocks], kv_lens [rows], refs [pages]")
+    if any(t is not None and (t.dtype != torch.int32 or not t.is_contiguous()) for t in (block_table, refs, kv_lens)):
+        raise TypeError(f"{name}: the block table, the lengths and the counts are contiguous int32")
+    if page < 1:
+        raise ValueError(f"{name}: a page holds at least one token")
+    return block_table.shape[0], block_table.shape[1], refs.shape[0]
+
+
+def _rows(name: str, rows, device) -> torch.Tensor:
+    t = torch.as_tensor(rows, device=device)
+    if t.dim() != 1 or (t.dtype not in (torch.int32, torch.int64) and t.numel()):
+        raise ValueError(f"{name}: rows are a list or a 1-D tensor of whole numbers")
+    return t.to(torch.int32).contiguous()
+
+
+def fork_pages(block_table: torch.Tensor, kv_lens: torch.Tensor, refs: torch.Tensor, src, dst, page_size: int) -> None:
+    """Rows ``dst[i]`` of the block table become copies of rows ``src[i]``, in place and without moving data: they let go of what they held
+    and hold the pages of the source's tokens (``refs`` counts how many entries hold a page). All sources are read as they were before the
+    call, so rows can be exchanged; pairs with a row outside the table and all but the first pair of a destination are skipped. The page that the source's last token is in is shared too:
+    ``reserve_pages`` copies it for whoever writes next. src, dst: whole numbers [n], lists or tensors."""
+    R, W, N = _check_page_state("fork_pages", block_table, refs, kv_lens, page_size)
+    src, dst = _rows("fork_pages", src, block_table.device), _rows("fork_pages", dst, block_table.device)
+    if src.shape != dst.shape:
+        raise ValueError("fork_pages: as many sources as destinations")
+    _check_device("fork_pages", block_table, kv_lens, refs, src, dst)
+    n = src.shape[0]
+    if n:
+        scratch = torch.empty(n * (W + 1), dtype=torch.int32, device=block_table.device)
+        _lib.call("b200_fork_pages", ptr(block_table), ptr(kv_lens), ptr(refs), ptr(src), ptr(dst), n, R, W, N, int(page_size), ptr(scratch), stream_ptr())
+        _count(2)
+
+
+def trim_pages(block_table: torch.Tensor, kv_lens: torch.Tensor, refs: torch.Tensor, page_size: int, lens: torch.Tensor | None = None, rows=None) -> None:
+    """Rows keep their first ``lens`` tokens (int32 [n]; None: none) and the pages of these, in place: drafts that were refused, sequences that are
+    over. ``rows`` [n] (default: all): which; a length below zero leaves a row alone, one above a row's length takes back unused room only."""
+    R, W, N = _check_page_state("trim_pages", block_table, refs, kv_lens, page_size)
+    rows = _rows("trim_pages", rows, block_table.device) if rows is not None else None
+    n = R if rows is None else rows.shape[0]
+    if lens is not None and (lens.dtype != torch.int32 or lens.shape != (n,) or not lens.is_contiguous()):
+        raise ValueError("trim_pages: one length (int32) for every row")
+    _check_device("trim_pages", block_table, kv_lens, refs, rows, lens)
+    if n:
+        _lib.call("b200_trim_pages", ptr(block_table), ptr(kv_lens), ptr(refs), ptr(rows), ptr(lens), n, R, W, N, int(page_size), stream_ptr())
+        _count()
+
+
+def reserve_pages(block_table: torch.Tensor, kv_lens: torch.Tensor, refs: torch.Tensor, count, caches, dim: int = 0,
+                  status: torch.Tensor | None = None) -> torch.Tensor:
+    """Room for ``count`` more tokens (a number, or int32 [rows]; rows with none are left alone) in every row, in place: the entries up to
+    ``ceil((kv_lens + count) / page)`` get free pages (in ascending order, row by row), and a row whose next token falls into a page that others hold
+    gets a copy of it (where all its holders ask, the first row keeps it). ``caches``: the tensors that the pages are in, ``[pages, tokens, ...]`` or
+    with ``dim=1`` ``[layers, pages, tokens, ...]``. Lengths stay as they are.
+
+    Returns ``status`` (int32 [1], on the device): 0, or 1 where too few pages are free and 2 where a row would outgrow the table; then nothing has
+    been changed."""
+    caches, tensors, page = _page_tensors("reserve_pages", caches, dim, refs.numel())
+    if not caches:
+        raise ValueError("reserve_pages: the caches that hold the pages are needed")
+    R, W, N = _check_page_state("reserve_pages", block_table, refs, kv_lens, page)
+    counts = None
+    if isinstance(count, torch.Tensor):
+        counts, count = count, 0
+        if counts.dtype != torch.int32 or counts.shape != (R,) or not counts.is_contiguous():
+            raise ValueError("reserve_pages: one count (int32) for every row")
+    elif count < 0 or count >= 1 << 30:
+        raise ValueError("reserve_pages: the count of tokens is not negative")
+    if status is not None and (status.dtype != torch.int32 or status.numel() != 1):
+        raise ValueError("reserve_pages: the status is one int32")
+    _check_device("reserve_pages", block_table, kv_lens, refs, counts, status, *caches)
+    if status is None:
+        status = torch.empty(1, dtype=torch.int32, device=refs.device)
+    scratch = torch.empty(8 * (R + N) + 16, dtype=torch.int32, device=refs.device)   # b200_pages_scratch
+    _lib.call("b200_reserve_pages", ptr(block_table), ptr(kv_lens), ptr(refs), ptr(counts), int(count), R, W, N, page, tensors, len(caches), ptr(scratch),
+              ptr(status), stream_ptr())
+    _count(2)
+    return status
+
+
+def compact_pages(block_table: torch.Tensor, refs: torch.Tensor, caches, dim: int = 0,
+                  out: tuple[torch.Tensor, torch.Tensor] | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+    """The pages in use move to the front of the caches (see ``reserve_pages``): those behind the first n (n: pages in use), in ascending order, to the
+    free ones among these. Returns the new (block_table, refs); ``out`` may be the old ones. The caches are changed in place."""
+    caches, tensors, page = _page_tensors("compact_pages", caches, dim, refs.numel())
+    R, W, N = _check_page_state("compact_pages", block_table, refs)
+    if out is None:
+        out = torch.empty_like(block_table), torch.empty_like(refs)
+    elif out[0].shape != block_table.shape or out[1].shape != refs.shape or any(t.dtype != torch.int32 or not t.is_contiguous() for t in out):
+        raise ValueError("compact_pages: the new tables are laid out like the old ones")
+    _check_device("compact_pages", block_table, refs, *out, *caches)
+    scratch = torch.empty(8 * (R + N) + 16, dtype=torch.int32, device=refs.device)
+    _lib.call("b200_compact_pages", ptr(block_table), ptr(out[0]), ptr(refs), ptr(out[1]), R, W, N, page or 1, tensors, len(caches), ptr(scratch), stream_ptr())
+    _count(2)
+    return out
+
+
+def copy_pages(caches, src: list[int], dst: list[int], dim: int = 0, tokens: list[int] | None = None) -> None:
+    """Pages ``src[i]`` are copied to ``dst[i]`` in all caches (see ``reserve_pages``), their first ``tokens[i]`` tokens alone where given. The page
+    numbers are lists on the host, which are looked at: in range, no destination twice, none that is also a source."""
+    caches, tensors, page = _page_tensors("copy_pages", caches, dim)
+    src, dst = [int(x) for x in src], [int(x) for x in dst]
+    tokens = [page or 0] * len(src) if tokens is None else [int(x) for x in tokens]
+    if not caches or len(src) != len(dst) or len(tokens) != len(src):
+        raise ValueError("copy_pages: caches, and as many sources as destinations (and counts)")
+    N = min(t.shape[dim] for t in caches)
+    if any(not 0 <= x < N for x in src + dst) or any(not 0 <= n <= page for n in tokens):
+        raise ValueError("copy_pages: a page or a count of tokens is out of range")
+    if len(set(dst)) != len(dst) or set(dst) & set(src):
+        raise ValueError("copy_pages: a page is the destination of several copies, or of one and the source of another")
+    _check_device("copy_pages", *caches)
+    if src:
+        moves = torch.tensor([[s, d, n, 0] for s, d, n in zip(src, dst, tokens)], dtype=torch.int32).to(caches[0].device)
+        _lib.call("b200_copy_pages", tensors, len(caches), ptr(moves), len(src), N, stream_ptr())
+        _count()
