@@ -47,8 +47,20 @@ def _attention_case(c, **kw):
     (9, 1, 64, 1, 128, 16, 1500, 40),    # 64 heads on one KV head
 ])
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
-def test_shared_prefix_attention(B, T, Hq, Hkv, D, page, shared, own, dtype):
-    _attention_case(prefix_batch(B, T, Hq, Hkv, D, page, shared, own, dtype, seed=B + shared, device="cuda"))
+@pytest.mark.parametrize("variant", ["warp", "tc"])
+def test_shared_prefix_attention(B, T, Hq, Hkv, D, page, shared, own, dtype, variant):
+    if variant == "tc" and (shared == 0 or page in (7, 48)):
+        pytest.skip("refused: nothing is shared, or pages that no tile is made of")
+    _attention_case(prefix_batch(B, T, Hq, Hkv, D, page, shared, own, dtype, seed=B + shared, device="cuda"), variant=variant)
+
+
+@pytest.mark.parametrize("B,T,Hq,Hkv,D,page,shared", [
+    (1, 1, 1, 1, 64, 8, 1), (1, 1, 8, 8, 128, 16, 127), (2, 3, 16, 2, 128, 32, 128), (5, 1, 40, 8, 128, 64, 129), (3, 2, 128, 1, 64, 128, 256),
+    (7, 4, 28, 4, 128, 256, 385), (26, 1, 40, 8, 128, 16, 1111), (40, 1, 14, 2, 64, 64, 5000), (300, 1, 8, 1, 128, 128, 640), (25, 5, 5, 1, 64, 384, 1500),
+    (128, 1, 2, 2, 128, 8, 3000), (129, 1, 1, 1, 64, 64, 20000), (64, 1, 64, 8, 128, 16, 2047), (1, 1, 48, 1, 128, 64, 4096)])
+def test_shared_prefix_attention_tiles(B, T, Hq, Hkv, D, page, shared):
+    """The tensor-core kernel at one and at two tiles of rows, full and ragged steps, all page sizes, head groups that do not divide a tile."""
+    _attention_case(prefix_batch(B, T, Hq, Hkv, D, page, shared, 20, seed=B, device="cuda"), variant="tc")
 
 
 @pytest.mark.parametrize("T,shared", [(1, 200), (4, 200), (3, 64)])
@@ -57,7 +69,8 @@ def test_shared_prefix_attention_of_short_rows(T, shared, B):
     """Rows of the batch without a sequence, sequences shorter than the shared keys, fewer keys than new tokens."""
     lens = [shared + 9, 0, shared - 1, T - 1, shared + T - 1, 5] + [shared + i % 9 for i in range(6, B)]
     c = prefix_batch(B, T, 16, 2, 128, 16, shared, 9, lens=lens, device="cuda")
-    _attention_case(c)
+    for variant in ("warp", "tc"):
+        _attention_case(c, variant=variant)
 
 
 def test_shared_prefix_attention_of_an_own_table_and_strided_rows():
@@ -96,7 +109,10 @@ def test_pages_outside_the_cache_count_as_zeros():
     c = prefix_batch(3, 1, 8, 2, 64, 16, 70, 30, lens=[100, 96, 95], device="cuda")
     c["block_table"][1, 5] = c["k_cache"].shape[0] + 5
     c["block_table"][2, 5] = -7
-    _attention_case(c)
+    c["block_table"][0, 2] = -1     # (for all: the shared keys are read through the first table)
+    c["block_table"][1, 2] = c["block_table"][2, 2] = 10 ** 9
+    for variant in ("warp", "tc"):
+        _attention_case(c, variant=variant)
 
 
 def test_shared_prefix_attention_offsets_beyond_32_bits():
@@ -108,9 +124,10 @@ def test_shared_prefix_attention_offsets_beyond_32_bits():
     n = small["k_cache"].shape[0]
     k[-n:], v[-n:] = small["k_cache"], small["v_cache"]
     from triton_distributed_b200 import ops
-    want = ops.shared_prefix_attention(**small)
-    got = ops.shared_prefix_attention(**{**small, "k_cache": k, "v_cache": v, "block_table": small["block_table"] + (N - n)})
-    assert torch.equal(got, want)
+    for variant in ("warp", "tc"):
+        want = ops.shared_prefix_attention(**small, variant=variant)
+        got = ops.shared_prefix_attention(**{**small, "k_cache": k, "v_cache": v, "block_table": small["block_table"] + (N - n)}, variant=variant)
+        assert torch.equal(got, want)
 
 
 def _same(got, want):

@@ -1,6 +1,7 @@
 // What the kernels of the shared-prefix attention (shared_prefix.cu, shared_prefix_sm100.cu) are told.
 #pragma once
 #include <cstdint>
+#include <cuda_runtime.h>
 
 namespace b200 {
 
@@ -18,10 +19,13 @@ struct SharedPrefixParams {
   int bt_stride, width, B, T, Hq, Hkv, num_blocks, page;
   int shared;               // keys that all sequences begin with
   int prefix_splits, own_splits, S;   // ranges of keys per row: S = prefix_splits + own_splits
-  int prefix_chunk;         // keys per range of the shared ones, a multiple of 64
+  int prefix_chunk;         // keys per CTA of the shared ones, a multiple of 64 (span kernel) or 128
   int prefix_ctas;          // CTAs of the shared keys in the span kernel's grid
   int late_wait;            // the kernel in front is this call's own: only the end of the span kernel waits for it
   float scale_log2e;        // softmax scale * log2(e)
 };
+
+bool shared_prefix_tc_takes(const SharedPrefixParams& p, int D);
+int shared_prefix_tc_launch(const SharedPrefixParams& p, int D, int dtype, cudaStream_t s);
 
 }  // namespace b200

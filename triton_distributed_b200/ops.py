@@ -981,21 +981,34 @@ def _check_device(name: str, *tensors: torch.Tensor | None) -> None:
 
 
 @functools.lru_cache(maxsize=1024)
-def choose_prefix_splits(batch: int, tokens: int, heads: int, kv_heads: int, shared: int, own: int, sm_count: int = 148) -> tuple[int, int]:
-    """Ranges of keys (of the shared keys, of everybody's own) for `shared_prefix_attention`: one wave of two CTAs per SM, all with about
-    as many keys, at least 128."""
+def choose_prefix_splits(batch: int, tokens: int, heads: int, kv_heads: int, shared: int, own: int, page: int = 64, slots: int = 0,
+                         sm_count: int = 148, variant: str | None = None) -> tuple[bool, int, int]:
+    """(tensor-core kernel for the shared keys, ranges of the shared keys, ranges of everybody's own keys) for `shared_prefix_attention`.
+
+    Warp kernel: one wave of two CTAs per SM, all with about as many keys, at least 128. Tensor-core kernel: the number of ranges with the least
+    waves times steps of 128 keys, where a CTA's start and end cost about three steps."""
     group = heads // kv_heads
     rows = batch * tokens * group
-    prefix_ctas = kv_heads * -(-rows // (32 if rows > 16 else 16)) if shared else 0
     own_ctas = batch * kv_heads * -(-tokens * group // (32 if tokens * group > 16 else 16))
+    able = shared > 0 and group <= 128 and page >= 8 and (page % 128 == 0 or 128 % page == 0) and slots < 0x7fffff00 and kv_heads <= 65535
+    if variant == "tc" and not able:
+        raise ValueError("shared_prefix_attention: these heads or pages are not for the tensor-core kernel")
+    tc = able and (rows > 32 if variant is None else variant == "tc")
+    prefix_ctas = kv_heads * -(-rows // (32 if rows > 16 else 16)) if shared and not tc else 0
     share = max(128, (prefix_ctas * shared + own_ctas * own) // (2 * sm_count))
     chunk = -(-share // 64) * 64
-    return (min(64, -(-shared // chunk)) if shared else 0), max(1, min(64, -(-own // chunk)))
+    own_splits = max(1, min(64, -(-own // chunk)))
+    if not tc:
+        return False, min(64, -(-shared // chunk)) if shared else 0, own_splits
+    tiles = -(-batch * tokens // (128 // group))
+    units, steps = kv_heads * -(-tiles // 2), -(-shared // 128)
+    best = min((-(-units * r // sm_count) * (-(-steps // r) + 3), r) for r in range(1, min(steps, 64) + 1))[1]
+    return True, best * (2 if tiles == 1 else 1), own_splits
 
 
 def shared_prefix_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, kv_lens: torch.Tensor, block_table: torch.Tensor,
                             shared: int, scale: float, tokens: int = 1, prefix_table: torch.Tensor | None = None, max_kv_len: int | None = None,
-                            out: torch.Tensor | None = None, return_lse: bool = False):
+                            out: torch.Tensor | None = None, return_lse: bool = False, variant: str | None = None):
     """Paged causal attention of the last `tokens` tokens of every sequence, where the first `shared` keys of all sequences are the same and
     are read once for the whole batch: several samples of one prompt, questions about one document, drafted tokens (``tokens`` > 1).
 
@@ -1004,7 +1017,8 @@ def shared_prefix_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: tor
     without any gives zeros. Keys j < ``shared`` are read through ``prefix_table`` (int32 [>= ceil(shared / page)], default: the first
     sequence's row of the block table) for every sequence that reaches beyond them with all its tokens; shorter sequences (also
     kv_lens 0) are attended over their own table alone. ``shared`` need not be a multiple of the page. ``max_kv_len``: an upper bound on kv_lens for the choice
-    of splits (default: what the table can hold). Returns [B * tokens, Hq, D] (and the natural-log LSE fp32 [B * tokens, Hq])."""
+    of splits (default: what the table can hold). ``variant``: which kernel reads the shared keys, "warp" (warp-level products, any page) or "tc" (tcgen05 tiles; pages
+    that 128 is a multiple of, or that are multiples of 128); None picks by the rows per KV head. Returns [B * tokens, Hq, D] (and the natural-log LSE fp32 [B * tokens, Hq])."""
     if q.dim() != 3 or k_cache.dim() != 4 or k_cache.shape != v_cache.shape or kv_lens.dim() != 1 or block_table.dim() != 2:
         raise ValueError("shared_prefix_attention: q [B * tokens, Hq, D], caches [num_blocks, page, Hkv, D], kv_lens [B], block_table [B, max_blocks]")
     T, Hq, D = q.shape
@@ -1013,6 +1027,8 @@ def shared_prefix_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: tor
     shared, tokens = int(shared), int(tokens)
     if q.dtype not in (torch.bfloat16, torch.float16) or k_cache.dtype != q.dtype or v_cache.dtype != q.dtype:
         raise TypeError("shared_prefix_attention handles bf16 / f16 (q and caches of one type)")
+    if variant not in (None, "tc", "warp"):
+        raise ValueError(f"shared_prefix_attention: variant {variant!r}")
     if D not in (64, 128) or Dk != D:
         raise ValueError(f"shared_prefix_attention: head sizes 64 and 128, got {D} and {Dk}")
     if tokens < 1 or T != B * tokens or kv_lens.shape[0] != B or Hkv < 1 or Hq % Hkv or Hq < 1 or N < 1 or page < 1:
@@ -1038,15 +1054,15 @@ def shared_prefix_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: tor
     lse = torch.empty((T, Hq), dtype=torch.float32, device=q.device) if return_lse else None
     if B:
         longest = width * page if max_kv_len is None else min(int(max_kv_len), width * page)
-        prefix_splits, own_splits = choose_prefix_splits(B, tokens, Hq, Hkv, shared, max(1, longest - shared))
+        tc, prefix_splits, own_splits = choose_prefix_splits(B, tokens, Hq, Hkv, shared, max(1, longest - shared), page, N * page, variant=variant)
         ranges = T * Hq * (prefix_splits + own_splits)
         part = torch.empty(ranges * (D + 1), dtype=torch.float32, device=q.device)   # outputs of all ranges, then their log-sum-exps
         at = part.data_ptr()
         _lib.call("b200_shared_prefix_attention", ptr(q), ctypes.c_longlong(q.stride(0) if T > 1 else Hq * D), ptr(k_cache), ptr(v_cache), ptr(kv_lens),
                   ptr(block_table), block_table.stride(0), width, ptr(prefix_table), B, tokens, Hq, Hkv, D, N, page, shared, c_float(scale),
-                  prefix_splits, own_splits, ctypes.c_void_p(at), ctypes.c_void_p(at + ranges * D * 4), ptr(out), ptr(lse), dtype_code(q.dtype),
+                  int(tc), prefix_splits, own_splits, ctypes.c_void_p(at), ctypes.c_void_p(at + ranges * D * 4), ptr(out), ptr(lse), dtype_code(q.dtype),
                   ptr(_pipeline_status(q.device)), stream_ptr())
-        _count(2)
+        _count(3 if tc else 2)
     return (out, lse) if return_lse else out
 
 
