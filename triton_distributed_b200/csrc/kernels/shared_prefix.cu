@@ -7,10 +7,13 @@
 // A row (token and query head) is split over disjoint ranges of keys. Every range leaves its normalised output o_i and its
 // log-sum-exp l_i; the whole is sum_i exp(l_i - l) o_i with l = log sum_i exp(l_i).
 //
-// This file holds the kernel on warp-level products (m16n8k16): 16 or 32 rows that share a KV head per CTA, each of the four warps
-// streaming its own slices of 16 keys through a private ring of three (cp.async, no barrier of the CTA in the loop), its running
-// maximum, sum and output in registers. It takes the own keys of every sequence and, while the rows per KV head are few, the
-// shared keys; both in one launch, the shared ones first because their CTAs run longest. What bounds it is the read of the keys.
+// This file holds the kernel on warp-level products (m16n8k16) with the keys on the wide side: S^T [16 keys, 8 rows] = K Q^T and O^T [D, 8 rows]
+// += V^T P^T, for 8, 16 or 32 rows that share a KV head per CTA. Each of the four warps streams its own slices of 16 keys through a
+// private ring of three (cp.async, no barrier of the CTA in the loop), its running maximum, sum and output in registers; a slice without a
+// new maximum of any row rescales nothing (one vote). It takes the own keys of every sequence and, while the rows per KV head are few,
+// the shared keys; both in one launch, the shared ones first because their CTAs run longest. What bounds it is the read of the keys, and in short
+// sequences the latency of starting and merging. The first form, with the rows on the 16 rows of the product, took 1136 instructions a
+// slice and fetched them from beyond the instruction cache (86 us for the own keys of 64 sequences of 544 keys, 8 KV heads).
 // Many rows go to the tensor-core kernel in shared_prefix_sm100.cu.
 //
 // A sequence that does not reach beyond the shared keys (a row of the batch that holds none, or a shorter one) is attended by
@@ -33,8 +36,18 @@ constexpr int kSpanRing = 3;     // slices in flight per warp
 template <int D>
 constexpr int span_smem() { return 4 * kSpanRing * 2 * kSpanSlice * D * 2; }
 
-// The value rows of a slice in which some keys are masked for some rows (between drafted tokens): a masked key has weight zero, and
-// zero times an infinity or NaN must not reach the row. Tells whether the slice holds such a value.
+__device__ __forceinline__ float span_exp2(float x) {   // one instruction; -inf gives 0
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ uint32_t movmatrix_trans(uint32_t a) {
+  uint32_t d;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
+  return d;
+}
+
+// Whether a slice of values holds one that is not finite.
 template <bool BF16, int D>
 __device__ __forceinline__ bool slice_has_nonfinite(uint32_t vs, int lane) {
   uint32_t bad = 0;
@@ -49,16 +62,18 @@ __device__ __forceinline__ bool slice_has_nonfinite(uint32_t vs, int lane) {
   return __any_sync(0xffffffffu, bad != 0u);
 }
 
-// One CTA: NM x 16 rows of KV head `kvh` from row `row0` of a group of `rows`, over keys [t0, t1) of the pages in `table`. A row r of
+// One CTA: 8 NB rows of KV head `kvh` from row `row0` of a group of `rows`, over keys [t0, t1) of the pages in `table`. A row r of
 // the group is query token first_token + r / G, head kvh * G + r % G. `own`: the rows are one sequence's and see keys below `limit0` + r / G.
-template <bool BF16, int D, int NM>
-__device__ void span_body(const SharedPrefixParams& p, uint8_t* smem, int kvh, int first_token, int row0, int rows, const int* table, int width,
-                          int t0, int t1, bool own, int limit0, int split) {
+template <bool BF16, int D, int NB>
+__device__ __forceinline__ void span_body(const SharedPrefixParams& p, uint8_t* smem, int kvh, int first_token, int row0, int rows, const int* table,
+                                          int width, int t0, int t1, bool own, int limit0, int split) {
   constexpr int kKK = D / 16, kRowBytes = D * 2, kChunks = D / 8, kSliceBytes = kSpanSlice * kRowBytes;
+  constexpr int kLaneRows = 32 / kChunks;                  // keys that a warp copies with one instruction
+  constexpr int kCopies = kSpanSlice / kLaneRows;
   const int G = p.Hq / p.Hkv;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int r_lo = lane >> 2;
-  const int nrows = min(NM * 16, rows - row0);
+  const int row = lane >> 2, col = (lane & 3) * 2;         // of an accumulator tile: key (or output column), row of the group and the next
+  const int nrows = min(NB * 8, rows - row0);
   auto row_id = [&](int r) {   // of row r of this CTA, among all rows of the call
     const int g = row0 + r;
     return static_cast<size_t>(first_token + g / G) * p.Hq + kvh * G + g % G;
@@ -68,188 +83,191 @@ __device__ void span_body(const SharedPrefixParams& p, uint8_t* smem, int kvh, i
     return;
   }
 
-  // ---- query fragments; rows that do not exist are zero ----
-  uint32_t qa[NM][kKK][4];
-  int limit[NM][2];
-#pragma unroll
-  for (int m = 0; m < NM; ++m)
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const int r = m * 16 + r_lo + 8 * h, g = row0 + r;
-      const bool in = r < nrows;
-      limit[m][h] = own ? min(t1, limit0 + g / G) : t1;
-      const uint32_t* src = reinterpret_cast<const uint32_t*>(static_cast<const uint8_t*>(p.q) + (static_cast<size_t>(first_token + g / G) * p.ldq +
-                                                              static_cast<size_t>(kvh * G + g % G) * D) * 2) + (lane & 3);
-#pragma unroll
-      for (int kk = 0; kk < kKK; ++kk) {
-        qa[m][kk][h] = in ? src[kk * 8] : 0u;
-        qa[m][kk][h + 2] = in ? src[kk * 8 + 4] : 0u;
-      }
-    }
-
   // ---- this warp's ring: slot s holds K at +0 and V behind it; slices begin at multiples of 16 keys ----
   const uint32_t ring = static_cast<uint32_t>(__cvta_generic_to_shared(smem)) + warp * (kSpanRing * 2 * kSliceBytes);
   const uint8_t *kc = static_cast<const uint8_t*>(p.k_cache), *vc = static_cast<const uint8_t*>(p.v_cache);
   const int base = t0 & ~(kSpanSlice - 1);
   const int n_slices = (t1 - base + kSpanSlice - 1) / kSpanSlice;
   const int mine = n_slices > warp ? (n_slices - warp + 3) / 4 : 0;   // slices warp, warp + 4, ...
-  const bool page_fast = p.page % kSpanSlice == 0;
-  auto page_of = [&](int tok) -> long long {   // first slot of the page that holds a token, or -1
+  const bool page_fast = p.page % kSpanSlice == 0;                    // a slice lies in one page
+  auto page_of = [&](int tok) -> int {   // -1: there is none
     const int w = tok / p.page;
     const int blk = w < width ? table[w] : -1;
-    return blk >= 0 && blk < p.num_blocks ? static_cast<long long>(blk) * p.page : -1;
+    return blk < p.num_blocks ? blk : -1;
   };
+  const int hi = lane / kChunks, chunk = lane % kChunks;
+  const size_t token_bytes = static_cast<size_t>(p.Hkv) * kRowBytes, step = token_bytes * kLaneRows;
+  const size_t lane_off = hi * token_bytes + static_cast<size_t>(kvh) * kRowBytes + chunk * 16;
+  int next_blk = page_fast && mine > 0 ? page_of(base + warp * kSpanSlice) : 0;   // one slice ahead of its copies
   auto load_slice = [&](int j) {   // always commits a group, so that the counting stays uniform
     if (j < mine) {
       const int st0 = base + (warp + 4 * j) * kSpanSlice;
       const uint32_t slot = ring + (j % kSpanRing) * (2 * kSliceBytes);
-      const long long first = page_fast ? page_of(st0) : 0;
+      const int blk = next_blk;
+      if (page_fast && j + 1 < mine) next_blk = page_of(st0 + 4 * kSpanSlice);
+      if (page_fast && blk >= 0 && st0 >= t0 && st0 + kSpanSlice <= t1) {
+        const size_t off = (static_cast<size_t>(blk) * p.page + st0 % p.page) * token_bytes + lane_off;
+        const uint8_t *ks = kc + off, *vs = vc + off;
 #pragma unroll
-      for (int i = 0; i < kSpanSlice * kChunks / 32; ++i) {
-        const int tok_in = (i * 32 + lane) / kChunks, c = lane % kChunks;
-        const int tok = st0 + tok_in;
-        bool valid = tok >= t0 && tok < t1;
-        long long page0 = first;
-        if (!page_fast && valid) page0 = page_of(tok);
-        valid = valid && page0 >= 0;
-        const size_t off = valid ? ((static_cast<size_t>(page0 + tok % p.page) * p.Hkv + kvh) * D + c * 8) * 2 : 0;
-        const uint32_t so = tok_in * kRowBytes + ((c ^ (tok_in & 7)) * 16);
-        cp_async_16(slot + so, kc + off, valid ? 16 : 0);
-        cp_async_16(slot + kSliceBytes + so, vc + off, valid ? 16 : 0);
+        for (int i = 0; i < kCopies; ++i) {
+          const int tok_in = i * kLaneRows + hi;
+          const uint32_t at = slot + tok_in * kRowBytes + ((chunk ^ (tok_in & 7)) * 16);
+          cp_async_16(at, ks + i * step, 16);
+          cp_async_16(at + kSliceBytes, vs + i * step, 16);
+        }
+      } else {
+#pragma unroll 1
+        for (int i = 0; i < kCopies; ++i) {
+          const int tok_in = i * kLaneRows + hi, tok = st0 + tok_in;
+          const int page = tok >= t0 && tok < t1 ? page_of(tok) : -1;
+          const size_t off = page >= 0 ? (static_cast<size_t>(page) * p.page + tok % p.page) * token_bytes + lane_off - hi * token_bytes : 0;
+          const uint32_t at = slot + tok_in * kRowBytes + ((chunk ^ (tok_in & 7)) * 16);
+          cp_async_16(at, kc + off, page >= 0 ? 16 : 0);
+          cp_async_16(at + kSliceBytes, vc + off, page >= 0 ? 16 : 0);
+        }
       }
     }
     cp_async_commit();
   };
-
-  float m_run[NM][2], l_run[NM][2], oacc[NM][2 * kKK][4];
-#pragma unroll
-  for (int m = 0; m < NM; ++m) {
-#pragma unroll
-    for (int h = 0; h < 2; ++h) { m_run[m][h] = -INFINITY; l_run[m][h] = 0.f; }
-#pragma unroll
-    for (int i = 0; i < 2 * kKK; ++i)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) oacc[m][i][e] = 0.f;
-  }
-  const int safe = own ? min(t1, limit0 + row0 / G) : t1;   // keys below are visible to every row of this CTA
 #pragma unroll
   for (int j = 0; j < kSpanRing - 1; ++j) load_slice(j);
+
+  // ---- Q^T fragments: row nb * 8 + lane / 4, elements 16 kk + col, + 1 and eight further; rows that do not exist are zero ----
+  uint32_t qb[NB][kKK][2];
+#pragma unroll
+  for (int nb = 0; nb < NB; ++nb) {
+    const int g = row0 + nb * 8 + row;
+    const bool in = nb * 8 + row < nrows;
+    const uint32_t* src = reinterpret_cast<const uint32_t*>(static_cast<const uint8_t*>(p.q) + (static_cast<size_t>(first_token + g / G) * p.ldq +
+                                                            static_cast<size_t>(kvh * G + g % G) * D) * 2) + (lane & 3);
+#pragma unroll
+    for (int kk = 0; kk < kKK; ++kk) {
+      qb[nb][kk][0] = in ? src[kk * 8] : 0u;
+      qb[nb][kk][1] = in ? src[kk * 8 + 4] : 0u;
+    }
+  }
+  int limit[NB][2];   // of rows nb * 8 + col, + 1
+#pragma unroll
+  for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+    for (int h = 0; h < 2; ++h) limit[nb][h] = own ? min(t1, limit0 + (row0 + nb * 8 + col + h) / G) : t1;
+  const int safe = own ? min(t1, limit0 + row0 / G) : t1;   // keys below are visible to every row of this CTA
+
+  float m_run[NB][2], l_run[NB][2], oacc[NB][kKK][4];   // of rows col, col + 1; l_run: this lane's keys; oacc: columns 16 dn + row (and + 8)
+#pragma unroll
+  for (int nb = 0; nb < NB; ++nb) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) { m_run[nb][h] = -INFINITY; l_run[nb][h] = 0.f; }
+#pragma unroll
+    for (int i = 0; i < kKK; ++i)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) oacc[nb][i][e] = 0.f;
+  }
+  const int mi = lane >> 3, mr = lane & 7;
+  const uint32_t k_row = ((mi & 1) * 8 + mr) * kRowBytes, v_row = ((mi >> 1) * 8 + mr) * kRowBytes;
+#pragma unroll 1
   for (int j = 0; j < mine; ++j) {
     load_slice(j + kSpanRing - 1);       // into the slot of the iteration before
     cp_async_wait<kSpanRing - 1>();      // this lane's part of slice j has landed; the barrier covers the other lanes
     __syncwarp();
     const uint32_t ks = ring + (j % kSpanRing) * (2 * kSliceBytes), vs = ks + kSliceBytes;
     const int st0 = base + (warp + 4 * j) * kSpanSlice;
-    // ---- scores of 16 keys ----
-    float s[NM][2][4];
+    // ---- S^T of 16 keys; for one block of rows two sums, so that no product waits for the one before it ----
+    constexpr int kSums = NB == 1 ? 2 : 1;
+    float s[NB][kSums][4];
 #pragma unroll
-    for (int m = 0; m < NM; ++m)
+    for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) s[m][0][e] = s[m][1][e] = 0.f;
+      for (int x = 0; x < kSums; ++x)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[nb][x][e] = 0.f;
 #pragma unroll
     for (int kk = 0; kk < kKK; ++kk) {
-      const int mat = lane >> 3, tok_in = (mat >> 1) * 8 + (lane & 7), c = 2 * kk + (mat & 1);
-      uint32_t b0, b1, b2, b3;
-      ldmatrix_x4(ks + tok_in * kRowBytes + ((c ^ (tok_in & 7)) * 16), b0, b1, b2, b3);
+      uint32_t a[4];
+      ldmatrix_x4(ks + k_row + (((2 * kk + (mi >> 1)) ^ mr) * 16), a[0], a[1], a[2], a[3]);
 #pragma unroll
-      for (int m = 0; m < NM; ++m) {
-        mma16816<BF16>(s[m][0], qa[m][kk], b0, b1);
-        mma16816<BF16>(s[m][1], qa[m][kk], b2, b3);
-      }
+      for (int nb = 0; nb < NB; ++nb) mma16816<BF16>(s[nb][kk % kSums], a, qb[nb][kk][0], qb[nb][kk][1]);
     }
     const bool whole = st0 >= t0 && st0 + kSpanSlice <= safe;
-    uint32_t pa[NM][4];
+    float v[NB][4];   // keys row, row, row + 8, row + 8 of rows col, col + 1, col, col + 1
+    bool raise = false;
 #pragma unroll
-    for (int m = 0; m < NM; ++m) {
+    for (int nb = 0; nb < NB; ++nb) {
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        float mx = -INFINITY;
+      for (int e = 0; e < 4; ++e) v[nb][e] = (kSums == 2 ? s[nb][0][e] + s[nb][kSums - 1][e] : s[nb][0][e]) * p.scale_log2e;
+      if (!whole) {
 #pragma unroll
-        for (int nb = 0; nb < 2; ++nb)
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            float v = s[m][nb][2 * h + e] * p.scale_log2e;
-            const int tok = st0 + nb * 8 + (lane & 3) * 2 + e;
-            if (!whole && (tok < t0 || tok >= limit[m][h])) v = -INFINITY;
-            s[m][nb][2 * h + e] = v;
-            mx = fmaxf(mx, v);
-          }
-        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-        const float m_new = fmaxf(m_run[m][h], mx);
-        const float ref = m_new == -INFINITY ? 0.f : m_new;
-        const float corr = exp2f(m_run[m][h] - ref);   // -inf -> 0
-        m_run[m][h] = m_new;
-        float sum = 0.f;
-#pragma unroll
-        for (int nb = 0; nb < 2; ++nb)
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            const float w = exp2f(s[m][nb][2 * h + e] - ref);
-            s[m][nb][2 * h + e] = w;
-            sum += w;
-          }
-        l_run[m][h] = l_run[m][h] * corr + sum;
-#pragma unroll
-        for (int i = 0; i < 2 * kKK; ++i) {
-          oacc[m][i][2 * h] *= corr;
-          oacc[m][i][2 * h + 1] *= corr;
+        for (int e = 0; e < 4; ++e) {
+          const int tok = st0 + row + 8 * (e >> 1);
+          if (tok < t0 || tok >= limit[nb][e & 1]) v[nb][e] = -INFINITY;
         }
       }
-      // the weights are rounded to the type of the values: the product's A operand has it (the row's largest is one, exactly)
 #pragma unroll
-      for (int nb = 0; nb < 2; ++nb)
+      for (int h = 0; h < 2; ++h) raise |= fmaxf(v[nb][h], v[nb][h + 2]) > m_run[nb][h];
+    }
+    if (__any_sync(0xffffffffu, raise)) {
 #pragma unroll
-        for (int h = 0; h < 2; ++h)
-          pa[m][nb * 2 + h] = BF16 ? pack_bf16x2(s[m][nb][2 * h], s[m][nb][2 * h + 1]) : pack_f16x2(s[m][nb][2 * h], s[m][nb][2 * h + 1]);
+      for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          float mx = fmaxf(v[nb][h], v[nb][h + 2]);
+#pragma unroll
+          for (int m = 4; m < 32; m <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, m));
+          const float m_new = fmaxf(m_run[nb][h], mx);
+          const float corr = m_new == -INFINITY ? 0.f : span_exp2(m_run[nb][h] - m_new);   // m_run = -inf -> 0
+          m_run[nb][h] = m_new;
+          l_run[nb][h] *= corr;
+#pragma unroll
+          for (int i = 0; i < kKK; ++i) {
+            oacc[nb][i][h] *= corr;
+            oacc[nb][i][2 + h] *= corr;
+          }
+        }
+    }
+    // the weights are rounded to the type of the values: the product's operand has it (a row's largest is one, exactly)
+    uint32_t pb[NB][2];
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb) {
+      float w[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) w[e] = span_exp2(v[nb][e] - (m_run[nb][e & 1] == -INFINITY ? 0.f : m_run[nb][e & 1]));
+      l_run[nb][0] += w[0] + w[2];
+      l_run[nb][1] += w[1] + w[3];
+#pragma unroll
+      for (int x = 0; x < 2; ++x) pb[nb][x] = movmatrix_trans(BF16 ? pack_bf16x2(w[2 * x], w[2 * x + 1]) : pack_f16x2(w[2 * x], w[2 * x + 1]));
     }
     if (!whole && own && slice_has_nonfinite<BF16, D>(vs, lane)) {
-      // ---- rare: what is not finite is added for the rows that see its key, and is zero in the product. The weights go through the
-      // slice's K slot, which has been used. ----
-      __syncwarp();
-      const uint32_t smem0 = static_cast<uint32_t>(__cvta_generic_to_shared(smem));
-      float* w_sh = reinterpret_cast<float*>(smem + (ks - smem0));   // [16 rows][16 keys]
-      uint8_t* v_sh = smem + (vs - smem0);
-      constexpr uint32_t kExp = BF16 ? 0x7f80u : 0x7c00u;
-#pragma unroll
-      for (int m = 0; m < NM; ++m) {
-#pragma unroll
-        for (int nb = 0; nb < 2; ++nb)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) w_sh[(r_lo + 8 * (e >> 1)) * 16 + nb * 8 + (lane & 3) * 2 + (e & 1)] = s[m][nb][e];
-        __syncwarp();
+      // ---- rare: between drafted tokens a key is masked for some rows, and zero times an infinity or NaN must not reach them. Token by
+      // token from the last one on: the keys that it does not see are zeroed, and the product is kept for its rows alone. ----
+      const int t_first = row0 / G, t_last = (row0 + nrows - 1) / G;
 #pragma unroll 1
-        for (int key = 0; key < kSpanSlice; ++key) {
-          const float w0 = w_sh[r_lo * 16 + key], w1 = w_sh[(r_lo + 8) * 16 + key];
+      for (int t = t_last; t >= t_first; --t) {
+        const int seen = max(0, min(kSpanSlice, min(t1, limit0 + t) - st0));
+        __syncwarp();
+        for (int i = seen * kChunks + lane; i < kSpanSlice * kChunks; i += 32)
+          asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(vs + i * 16), "r"(0u) : "memory");
+        __syncwarp();
 #pragma unroll
-          for (int i = 0; i < 2 * kKK; ++i) {
-            const uint32_t raw = *reinterpret_cast<const uint32_t*>(v_sh + key * kRowBytes + ((i ^ (key & 7)) * 16) + (lane & 3) * 4);
-            const float2 v = BF16 ? unpack_bf16x2(raw) : unpack_f16x2(raw);
-            const bool x = (raw & kExp) == kExp, y = (raw >> 16 & kExp) == kExp;
-            if (x && w0 > 0.f) oacc[m][i][0] += w0 * v.x;
-            if (y && w0 > 0.f) oacc[m][i][1] += w0 * v.y;
-            if (x && w1 > 0.f) oacc[m][i][2] += w1 * v.x;
-            if (y && w1 > 0.f) oacc[m][i][3] += w1 * v.y;
+        for (int dn = 0; dn < kKK; ++dn) {
+          uint32_t a[4];
+          ldmatrix_x4_trans(vs + v_row + (((2 * dn + (mi & 1)) ^ mr) * 16), a[0], a[1], a[2], a[3]);
+#pragma unroll
+          for (int nb = 0; nb < NB; ++nb) {
+            float d[4] = {oacc[nb][dn][0], oacc[nb][dn][1], oacc[nb][dn][2], oacc[nb][dn][3]};
+            mma16816<BF16>(d, a, pb[nb][0], pb[nb][1]);
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              if ((row0 + nb * 8 + col + (e & 1)) / G == t) oacc[nb][dn][e] = d[e];
           }
         }
-        __syncwarp();
       }
-      for (int i = lane; i < kSliceBytes / 4; i += 32) {
-        uint32_t* at = reinterpret_cast<uint32_t*>(v_sh) + i;
-        const uint32_t raw = *at;
-        *at = ((raw & kExp) == kExp ? 0u : raw & 0xffffu) | ((raw >> 16 & kExp) == kExp ? 0u : raw & 0xffff0000u);
-      }
-      __syncwarp();
-    }
+    } else {
 #pragma unroll
-    for (int dn = 0; dn < kKK; ++dn) {
-      const int mat = lane >> 3, tok_in = (mat & 1) * 8 + (lane & 7), c = 2 * dn + (mat >> 1);
-      uint32_t b0, b1, b2, b3;
-      ldmatrix_x4_trans(vs + tok_in * kRowBytes + ((c ^ (tok_in & 7)) * 16), b0, b1, b2, b3);
+      for (int dn = 0; dn < kKK; ++dn) {
+        uint32_t a[4];
+        ldmatrix_x4_trans(vs + v_row + (((2 * dn + (mi & 1)) ^ mr) * 16), a[0], a[1], a[2], a[3]);
 #pragma unroll
-      for (int m = 0; m < NM; ++m) {
-        mma16816<BF16>(oacc[m][2 * dn], pa[m], b0, b1);
-        mma16816<BF16>(oacc[m][2 * dn + 1], pa[m], b2, b3);
+        for (int nb = 0; nb < NB; ++nb) mma16816<BF16>(oacc[nb][dn], a, pb[nb][0], pb[nb][1]);
       }
     }
     __syncwarp();   // the slot is free for the copies of the next iteration
@@ -258,87 +276,89 @@ __device__ void span_body(const SharedPrefixParams& p, uint8_t* smem, int kvh, i
   __syncthreads();  // all rings are idle: their memory becomes the merge area
 
   // ---- merge of the four warps ----
-  float* red_m = reinterpret_cast<float*>(smem);     // [4][NM * 16]
-  float* red_l = red_m + 4 * NM * 16;                // [4][NM * 16]
-  float* red_o = red_l + 4 * NM * 16;                // [4][NM * 16][D]
+  constexpr int kRows = NB * 8, kPitch = D + 4;      // (lanes of one store are columns of four rows: 4 words apart in the banks)
+  float* red_m = reinterpret_cast<float*>(smem);     // [4][rows]
+  float* red_l = red_m + 4 * kRows;                  // [4][rows]
+  float* red_o = red_l + 4 * kRows;                  // [4][rows][pitch]
 #pragma unroll
-  for (int m = 0; m < NM; ++m)
+  for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      l_run[m][h] += __shfl_xor_sync(0xffffffffu, l_run[m][h], 1);
-      l_run[m][h] += __shfl_xor_sync(0xffffffffu, l_run[m][h], 2);
-      if ((lane & 3) == 0) {
-        red_m[(warp * NM + m) * 16 + r_lo + 8 * h] = m_run[m][h];
-        red_l[(warp * NM + m) * 16 + r_lo + 8 * h] = l_run[m][h];
+#pragma unroll
+      for (int m = 4; m < 32; m <<= 1) l_run[nb][h] += __shfl_xor_sync(0xffffffffu, l_run[nb][h], m);
+      const int r = warp * kRows + nb * 8 + col + h;
+      if (row == 0) { red_m[r] = m_run[nb][h]; red_l[r] = l_run[nb][h]; }
+      float* o = red_o + r * kPitch + row;
+#pragma unroll
+      for (int i = 0; i < kKK; ++i) {
+        o[16 * i] = oacc[nb][i][h];
+        o[16 * i + 8] = oacc[nb][i][2 + h];
       }
     }
-#pragma unroll
-  for (int m = 0; m < NM; ++m)
-#pragma unroll
-    for (int i = 0; i < 2 * kKK; ++i)
-#pragma unroll
-      for (int h = 0; h < 2; ++h)
-        *reinterpret_cast<float2*>(red_o + (static_cast<size_t>(warp * NM + m) * 16 + r_lo + 8 * h) * D + i * 8 + (lane & 3) * 2) =
-            make_float2(oacc[m][i][2 * h], oacc[m][i][2 * h + 1]);
   __syncthreads();
-  for (int i = threadIdx.x; i < nrows * D; i += kSpanThreads) {
-    const int r = i / D, c = i - r * D;
+  constexpr int kVecs = D / 4;
+  for (int i = threadIdx.x; i < nrows * kVecs; i += kSpanThreads) {
+    const int r = i / kVecs, c = i - r * kVecs;
     float top = -INFINITY;
 #pragma unroll
-    for (int w = 0; w < 4; ++w) top = fmaxf(top, red_m[w * NM * 16 + r]);
-    float l = 0.f, o = 0.f;
+    for (int w = 0; w < 4; ++w) top = fmaxf(top, red_m[w * kRows + r]);
+    float l = 0.f;
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
     for (int w = 0; w < 4; ++w) {
-      const float mw = red_m[w * NM * 16 + r], f = mw == -INFINITY ? 0.f : exp2f(mw - top);   // (a sum that is NaN stays one)
-      l += red_l[w * NM * 16 + r] * f;
-      o += red_o[static_cast<size_t>(w * NM * 16 + r) * D + c] * f;
+      const float mw = red_m[w * kRows + r], f = mw == -INFINITY ? 0.f : span_exp2(mw - top);   // (a sum that is NaN stays one)
+      const float4 x = *reinterpret_cast<const float4*>(red_o + (w * kRows + r) * kPitch + c * 4);
+      l += red_l[w * kRows + r] * f;
+      o.x += x.x * f; o.y += x.y * f; o.z += x.z * f; o.w += x.w * f;
     }
     const size_t id = row_id(r) * p.S + split;
-    p.o_part[id * D + c] = l > 0.f ? o / l : (l == l ? 0.f : l);
+    const float inv = l > 0.f ? 1.f / l : (l == l ? 0.f : l);
+    *reinterpret_cast<float4*>(p.o_part + id * D + c * 4) = make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
     if (c == 0) p.lse_part[id] = l > 0.f ? top * 0.6931471805599453f + logf(l) : (l == l ? -INFINITY : l);
   }
 }
 
 // blockIdx.x: first the CTAs of the shared keys (split fastest, then row group, then KV head), then those of the own keys (split
 // fastest, then row group, KV head, sequence).
-template <bool BF16, int D, int NMP, int NMO>
+template <bool BF16, int D, int NBP, int NBO>
 __global__ void __launch_bounds__(kSpanThreads) shared_prefix_span_kernel(const SharedPrefixParams p) {
   extern __shared__ __align__(128) uint8_t smem[];
   if (!p.late_wait) griddep_wait();
   griddep_launch_dependents();
   const int G = p.Hq / p.Hkv;
   int at = blockIdx.x;
-  if (at < p.prefix_ctas) {
-    const int split = at % p.prefix_splits;
-    at /= p.prefix_splits;
-    const int groups = p.prefix_ctas / p.prefix_splits / p.Hkv;
-    const int kvh = at / groups, group = at % groups;
-    const int t0 = split * p.prefix_chunk, t1 = min(p.shared, t0 + p.prefix_chunk);
-    span_body<BF16, D, NMP>(p, smem, kvh, 0, group * NMP * 16, p.B * p.T * G, p.prefix_table, (p.shared + p.page - 1) / p.page, t0,
-                            t1, false, 0, split);
-    // rows of sequences that do not reach beyond the shared keys are attended by themselves
-    __syncthreads();
-    for (int r = threadIdx.x; r < NMP * 16; r += kSpanThreads) {
-      const int g = group * NMP * 16 + r;
-      if (g >= p.B * p.T * G) break;
-      const int token = g / G;
-      if (p.kv_lens[token / p.T] - p.T + 1 < p.shared) p.lse_part[(static_cast<size_t>(token) * p.Hq + kvh * G + g % G) * p.S + split] = -INFINITY;
+  if constexpr (NBP > 0) {
+    if (at < p.prefix_ctas) {
+      const int split = at % p.prefix_splits;
+      at /= p.prefix_splits;
+      const int groups = p.prefix_ctas / p.prefix_splits / p.Hkv;
+      const int kvh = at / groups, group = at % groups;
+      const int t0 = split * p.prefix_chunk, t1 = min(p.shared, t0 + p.prefix_chunk);
+      span_body<BF16, D, NBP>(p, smem, kvh, 0, group * NBP * 8, p.B * p.T * G, p.prefix_table, (p.shared + p.page - 1) / p.page, t0, t1, false, 0, split);
+      // rows of sequences that do not reach beyond the shared keys are attended by themselves
+      __syncthreads();
+      for (int r = threadIdx.x; r < NBP * 8; r += kSpanThreads) {
+        const int g = group * NBP * 8 + r;
+        if (g >= p.B * p.T * G) break;
+        const int token = g / G;
+        if (p.kv_lens[token / p.T] - p.T + 1 < p.shared) p.lse_part[(static_cast<size_t>(token) * p.Hq + kvh * G + g % G) * p.S + split] = -INFINITY;
+      }
+      return;
     }
-  } else {
-    at -= p.prefix_ctas;
-    const int split = at % p.own_splits;
-    at /= p.own_splits;
-    const int rows = p.T * G, groups = (rows + NMO * 16 - 1) / (NMO * 16);
-    const int group = at % groups;
-    at /= groups;
-    const int kvh = at % p.Hkv, b = at / p.Hkv;
-    const int len = max(0, p.kv_lens[b]), start = len - p.T + 1 >= p.shared ? p.shared : 0;
-    int chunk = (len - start + p.own_splits - 1) / p.own_splits;
-    chunk = (chunk + 4 * kSpanSlice - 1) / (4 * kSpanSlice) * (4 * kSpanSlice);
-    const int t0 = start + split * chunk, t1 = min(len, t0 + chunk);
-    span_body<BF16, D, NMO>(p, smem, kvh, b * p.T, group * NMO * 16, rows, p.block_table + static_cast<size_t>(b) * p.bt_stride, p.width, t0, t1,
-                            true, len - p.T + 1, p.prefix_splits + split);
   }
+  at -= p.prefix_ctas;
+  const int split = at % p.own_splits;
+  at /= p.own_splits;
+  const int rows = p.T * G, groups = (rows + NBO * 8 - 1) / (NBO * 8);
+  const int group = at % groups;
+  at /= groups;
+  const int kvh = at % p.Hkv, b = at / p.Hkv;
+  const int len = max(0, p.kv_lens[b]), start = len - p.T + 1 >= p.shared ? p.shared : 0;
+  int chunk = (len - start + p.own_splits - 1) / p.own_splits;
+  chunk = (chunk + 4 * kSpanSlice - 1) / (4 * kSpanSlice) * (4 * kSpanSlice);
+  const int t0 = start + split * chunk, t1 = min(len, t0 + chunk);
+  span_body<BF16, D, NBO>(p, smem, kvh, b * p.T, group * NBO * 8, rows, p.block_table + static_cast<size_t>(b) * p.bt_stride, p.width, t0, t1,
+                          true, len - p.T + 1, p.prefix_splits + split);
   if (p.late_wait) griddep_wait();   // the kernel in front (the shared keys') is complete before this one is
 }
 
@@ -382,12 +402,12 @@ __global__ void __launch_bounds__(128) shared_prefix_merge_kernel(const float* _
   if (lane == 0 && out_lse != nullptr) out_lse[row] = den > 0.f || den != den ? ref + logf(den) : -INFINITY;
 }
 
-template <bool BF16, int D, int NMP, int NMO>
+template <bool BF16, int D, int NBP, int NBO>
 static int launch_span(const SharedPrefixParams& p, int ctas, cudaStream_t s) {
   static bool configured[64] = {false};
   int dev = 0;
   B200_CHECK_CUDA(cudaGetDevice(&dev));
-  auto kernel = shared_prefix_span_kernel<BF16, D, NMP, NMO>;
+  auto kernel = shared_prefix_span_kernel<BF16, D, NBP, NBO>;
   if (!configured[dev & 63]) {
     B200_CHECK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, span_smem<D>()));
     configured[dev & 63] = true;
@@ -396,10 +416,16 @@ static int launch_span(const SharedPrefixParams& p, int ctas, cudaStream_t s) {
   return kOk;
 }
 
+// Blocks of eight rows per CTA for a number of rows: 1, 2 or 4.
+static int span_blocks(long long rows) { return rows <= 8 ? 1 : rows <= 16 ? 2 : 4; }
+
 template <int D>
-static int launch_span_form(const SharedPrefixParams& p, bool bf16, int nmp, int nmo, int ctas, cudaStream_t s) {
+static int launch_span_form(const SharedPrefixParams& p, bool bf16, int nbp, int nbo, int ctas, cudaStream_t s) {
 #define B200_SPAN(A, C) (bf16 ? launch_span<true, D, A, C>(p, ctas, s) : launch_span<false, D, A, C>(p, ctas, s))
-  return nmo == 2 ? B200_SPAN(2, 2) : nmp == 2 ? B200_SPAN(2, 1) : B200_SPAN(1, 1);
+  if (nbp == 0) return nbo == 1 ? B200_SPAN(0, 1) : nbo == 2 ? B200_SPAN(0, 2) : B200_SPAN(0, 4);
+  if (nbp == 1) return B200_SPAN(1, 1);
+  if (nbp == 2) return nbo == 1 ? B200_SPAN(2, 1) : B200_SPAN(2, 2);
+  return nbo == 1 ? B200_SPAN(4, 1) : nbo == 2 ? B200_SPAN(4, 2) : B200_SPAN(4, 4);
 #undef B200_SPAN
 }
 
@@ -433,7 +459,7 @@ B200_API int b200_shared_prefix_attention(const void* q, long long ldq, const vo
   const int G = Hq / Hkv;
   const long long prefix_rows = static_cast<long long>(B) * T * G, own_rows = static_cast<long long>(T) * G;
   B200_REQUIRE(prefix_rows * Hkv <= 1 << 30, "shared-prefix attention: too many rows");
-  const int nmp = prefix_rows > 16 ? 2 : 1, nmo = own_rows > 16 ? 2 : 1;
+  const int nbp = tc || shared == 0 ? 0 : span_blocks(prefix_rows), nbo = span_blocks(own_rows);
   long long ctas = 0;
   if (tc) {
     B200_REQUIRE(shared_prefix_tc_takes(p, D), "shared-prefix attention: these heads or pages are not for the tensor-core kernel");
@@ -446,13 +472,13 @@ B200_API int b200_shared_prefix_attention(const void* q, long long ldq, const vo
     p.late_wait = pdl_enabled();
   } else if (shared > 0) {
     p.prefix_chunk = ((shared + prefix_splits - 1) / prefix_splits + 63) / 64 * 64;
-    ctas = (prefix_rows + nmp * 16 - 1) / (nmp * 16) * Hkv * prefix_splits;
+    ctas = (prefix_rows + nbp * 8 - 1) / (nbp * 8) * Hkv * prefix_splits;
     p.prefix_ctas = static_cast<int>(ctas);
   }
-  ctas += (own_rows + nmo * 16 - 1) / (nmo * 16) * Hkv * B * own_splits;
+  ctas += (own_rows + nbo * 8 - 1) / (nbo * 8) * Hkv * B * own_splits;
   B200_REQUIRE(ctas <= 0x7fffffffLL, "shared-prefix attention: grid is too large");
-  const int rc = D == 128 ? launch_span_form<128>(p, dtype == kBF16, nmp, nmo, static_cast<int>(ctas), s)
-                          : launch_span_form<64>(p, dtype == kBF16, nmp, nmo, static_cast<int>(ctas), s);
+  const int rc = D == 128 ? launch_span_form<128>(p, dtype == kBF16, nbp, nbo, static_cast<int>(ctas), s)
+                          : launch_span_form<64>(p, dtype == kBF16, nbp, nbo, static_cast<int>(ctas), s);
   if (rc != kOk) return rc;
   const int rows = B * T * Hq;
 #define B200_MERGE(TT, DD)                                                                                                     \

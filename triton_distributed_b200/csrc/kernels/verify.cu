@@ -12,8 +12,9 @@
 // additions. Values that are not positive and finite count as zero, drafts outside the vocabulary are never accepted.
 //
 // A cluster of CTAs takes a sequence: all find n for themselves (a few loads), then every warp adds up its own contiguous run
-// of the one row (two with draft probabilities) that is needed, the CTAs exchange their sums through distributed shared memory,
-// and the warp whose interval holds the target walks its run once more, which the caches still have. One pass over memory.
+// of the one row (two with draft probabilities) that is needed and the CTAs write their sums into each other's shared memory. The CTA with
+// the warp whose interval holds the target cuts that run (which the caches still have) into a part for each warp, and the warp with the target walks its part. One
+// pass over memory.
 #include "b200/host.h"
 #include "b200/elem.cuh"
 #include "b200/primitives.cuh"
@@ -41,17 +42,106 @@ struct VerifyParams {
 
 __device__ __forceinline__ float probability(float x) { return x > 0.f && x < INFINITY ? x : 0.f; }
 
+// Elements that a lane reads at a time: 16 bytes where both rows start on 16 bytes, else one.
+template <typename T, int N>
+struct Lanes {
+  float v[N];
+  __device__ __forceinline__ void load(const T* p) {
+    if (N == 1) { v[0] = to_float(p[0]); return; }
+    const uint4 raw = *reinterpret_cast<const uint4*>(p);
+    const T* x = reinterpret_cast<const T*>(&raw);
+#pragma unroll
+    for (int e = 0; e < N; ++e) v[e] = to_float(x[e]);
+  }
+};
+
+// The weights of a row: max(p - q, 0) with q, p without the refused token otherwise.
 template <typename T>
+struct Weights {
+  const T* p;
+  const T* q;       // nullable
+  long long hole;   // a token without a weight, or -1
+  template <int N>
+  __device__ __forceinline__ void operator()(int j, double (&w)[N]) const {   // of tokens j ... j + N - 1
+    Lanes<T, N> a, b;
+    a.load(p + j);
+    if (q) b.load(q + j);
+#pragma unroll
+    for (int e = 0; e < N; ++e) {
+      w[e] = probability(a.v[e]);
+      if (q) w[e] = fmax(w[e] - static_cast<double>(probability(b.v[e])), 0.0);
+      else if (j + e == hole) w[e] = 0.0;
+    }
+  }
+};
+
+// The sum of the weights of [lo, hi) and the last token among them that has one (-1), by a warp; lo and hi are multiples of N but for the
+// row's end. Groups of loads before any of their values is used.
+template <typename T, int N>
+__device__ __forceinline__ double warp_mass(const Weights<T>& weights, int lo, int hi, int& last) {
+  constexpr int kStep = 32 * N, kGroup = N == 1 ? 8 : N == 8 ? 2 : 4;
+  const int lane = threadIdx.x & 31;
+  double sum[2] = {0.0, 0.0};
+  int j = lo + lane * N;
+  last = -1;
+  for (; j + (kGroup - 1) * kStep + N <= hi; j += kGroup * kStep) {
+    Lanes<T, N> a[kGroup], b[kGroup];
+#pragma unroll
+    for (int g = 0; g < kGroup; ++g) a[g].load(weights.p + j + g * kStep);
+    if (weights.q)
+#pragma unroll
+      for (int g = 0; g < kGroup; ++g) b[g].load(weights.q + j + g * kStep);
+#pragma unroll
+    for (int g = 0; g < kGroup; ++g)
+#pragma unroll
+      for (int e = 0; e < N; ++e) {
+        const int at = j + g * kStep + e;
+        const float x = probability(a[g].v[e]), y = weights.q ? probability(b[g].v[e]) : at == weights.hole ? x : 0.f;
+        // (of the difference's double rounding nothing is lost where the sign is decided in 32 bits: it is exact there)
+        if (x > y) {
+          sum[e & 1] += static_cast<double>(x) - static_cast<double>(y);
+          last = at;
+        }
+      }
+  }
+  for (; j < hi; j += kStep) {
+    if (j + N <= hi) {
+      double w[N];
+      weights(j, w);
+#pragma unroll
+      for (int e = 0; e < N; ++e)
+        if (w[e] > 0.0) { sum[e & 1] += w[e]; last = j + e; }
+    } else {
+      for (int e = 0; j + e < hi; ++e) {
+        double w[1];
+        weights(j + e, w);
+        if (w[0] > 0.0) { sum[0] += w[0]; last = j + e; }
+      }
+    }
+  }
+  double total = sum[0] + sum[1];
+#pragma unroll
+  for (int o = 16; o; o >>= 1) {
+    total += __shfl_xor_sync(0xffffffffu, total, o);
+    last = max(last, __shfl_xor_sync(0xffffffffu, last, o));
+  }
+  return total;
+}
+
+template <typename T, int N>
 __global__ void __launch_bounds__(kVerifyThreads) verify_drafts_kernel(const VerifyParams p) {
   namespace cg = cooperative_groups;
   cg::cluster_group cluster = cg::this_cluster();
-  __shared__ double warp_sum_of[kVerifyWarps];
-  __shared__ double x_total, all_total[kVerifyMaxCtas];
-  __shared__ int x_last, all_last[kVerifyMaxCtas];
-  __shared__ int s_accepted, s_last;
+  __shared__ double warp_sums[kVerifyWarps];
+  __shared__ int warp_last[kVerifyWarps];
+  __shared__ double all_total[2][kVerifyMaxCtas];   // written by all CTAs of the cluster, for each attempt
+  __shared__ int all_last[2][kVerifyMaxCtas];
+  __shared__ int s_accepted, s_run;
+  __shared__ double s_before;
   const int crank = static_cast<int>(cluster.block_rank()), csize = static_cast<int>(cluster.num_blocks());
   const int b = blockIdx.x / csize;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");   // the others' shared memory may be written once all have started
   griddep_wait();
   griddep_launch_dependents();
 
@@ -61,16 +151,18 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_drafts_kernel(const Ver
   const float* u_row = p.uniform + static_cast<size_t>(b) * (p.K + 1);
   const T* target = static_cast<const T*>(p.target) + b * p.t_b;
   const T* draft = p.draft ? static_cast<const T*>(p.draft) + b * p.d_b : nullptr;
+  const double u_last = u_row[p.K];
   if (warp == 0) {
     int n = 0;
     for (int k0 = 0; k0 < len; k0 += 32) {
       bool stands = false;
       if (k0 + lane < len) {
         const long long d = d_row[k0 + lane];
+        const double u = u_row[k0 + lane];
         if (d >= 0 && d < p.V) {
           const double pd = probability(to_float(target[(k0 + lane) * p.t_k + d]));
           const double qd = draft ? static_cast<double>(probability(to_float(draft[(k0 + lane) * p.d_k + d]))) : 1.0;
-          stands = static_cast<double>(u_row[k0 + lane]) * qd < pd;
+          stands = u * qd < pd;
         }
       }
       const uint32_t yes = __ballot_sync(0xffffffffu, stands);
@@ -78,66 +170,40 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_drafts_kernel(const Ver
       n += run;
       if (run < 32) break;
     }
-    if (lane == 0) s_accepted = n;
+    if (lane == 0) { s_accepted = n; s_run = -1; }
   }
   __syncthreads();
   const int n = s_accepted;
-  const T* pr = target + n * p.t_k;
   const bool rest = n < len;                                   // a draft was refused
-  const T* qr = rest && draft ? draft + n * p.d_k : nullptr;
-  const long long refused = rest && !draft ? d_row[n] : -1;    // has no weight
+  Weights<T> weights = {target + n * p.t_k, rest && draft ? draft + n * p.d_k : nullptr, rest && !draft ? d_row[n] : -1};
 
-  const int per_cta = (p.V + csize - 1) / csize;
-  const int per_warp = ((per_cta + kVerifyWarps - 1) / kVerifyWarps + 31) / 32 * 32;
-  const int c0 = min(p.V, crank * per_cta), c1 = min(p.V, c0 + per_cta);
-  const int lo = min(c1, c0 + warp * per_warp), hi = min(c1, lo + per_warp);
-  bool minus = true;   // subtract the draft's probabilities
-  auto weight = [&](int j) -> double {
-    double w = probability(to_float(pr[j]));
-    if (minus) {
-      if (qr) w = fmax(w - static_cast<double>(probability(to_float(qr[j]))), 0.0);
-      else if (j == refused) w = 0.0;
-    }
-    return w;
-  };
+  // CTA c takes [c * per_cta, ...), its warp w [w * per_warp, ...) of that; all but the row's end are multiples of 32 N
+  constexpr int kUnit = 32 * N;
+  const int per_warp = (p.V + csize * kVerifyWarps * kUnit - 1) / (csize * kVerifyWarps * kUnit) * kUnit;
+  const int lo = static_cast<int>(min(static_cast<long long>(p.V), (static_cast<long long>(crank) * kVerifyWarps + warp) * per_warp));
+  const int hi = min(p.V, lo + per_warp);
   // The edges of this warp's interval. Neighbours compute a common edge by the same additions, so the intervals have neither gaps nor
   // overlaps whatever the rounding.
   double before = 0.0, behind = 0.0, total = 0.0;
   int last = -1;
   for (int attempt = 0; attempt < 2; ++attempt) {
-    double sum = 0.0;
-    last = -1;   // the last token with a weight
-    for (int j = lo + lane; j < hi; j += 32) {
-      const double w = weight(j);
-      sum += w;
-      if (w > 0.0) last = j;
-    }
-#pragma unroll
-    for (int o = 16; o; o >>= 1) {
-      sum += __shfl_xor_sync(0xffffffffu, sum, o);
-      last = max(last, __shfl_xor_sync(0xffffffffu, last, o));
-    }
-    if (threadIdx.x == 0) s_last = -1;
-    __syncthreads();
-    if (lane == 0) {
-      warp_sum_of[warp] = sum;
-      atomicMax(&s_last, last);
-    }
+    int my_last;
+    const double sum = warp_mass<T, N>(weights, lo, hi, my_last);
+    if (lane == 0) { warp_sums[warp] = sum; warp_last[warp] = my_last; }
     __syncthreads();
     double in_cta = 0.0;
+    int cta_last = -1;
+#pragma unroll
     for (int w = 0; w < kVerifyWarps; ++w) {
       if (w == warp) before = in_cta;
-      in_cta += warp_sum_of[w];
+      in_cta += warp_sums[w];
       if (w == warp) behind = in_cta;
+      cta_last = max(cta_last, warp_last[w]);
     }
-    if (threadIdx.x == 0) {
-      x_total = in_cta;
-      x_last = s_last;
-    }
-    cluster.sync();
+    if (attempt == 0) asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
     if (threadIdx.x < csize) {
-      all_total[threadIdx.x] = *cluster.map_shared_rank(&x_total, threadIdx.x);
-      all_last[threadIdx.x] = *cluster.map_shared_rank(&x_last, threadIdx.x);
+      *cluster.map_shared_rank(&all_total[attempt][crank], threadIdx.x) = in_cta;
+      *cluster.map_shared_rank(&all_last[attempt][crank], threadIdx.x) = cta_last;
     }
     cluster.sync();
     total = 0.0;
@@ -145,35 +211,61 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_drafts_kernel(const Ver
     double front = 0.0;
     for (int c = 0; c < csize; ++c) {
       if (c == crank) front = total;
-      total += all_total[c];
-      last = max(last, all_last[c]);
+      total += all_total[attempt][c];
+      last = max(last, all_last[attempt][c]);
     }
     before += front;
     behind += front;
-    if (total > 0.0 || !rest || !minus) break;
-    minus = false;   // the target has nothing beyond the draft: its own probabilities
+    if (total > 0.0 || !rest || (weights.q == nullptr && weights.hole < 0)) break;
+    weights.q = nullptr;   // the target has nothing beyond the draft: its own probabilities
+    weights.hole = -1;
   }
 
-  // ---- the drawn token: the warp whose interval holds the target walks its run ----
-  const double aim = fmax(static_cast<double>(u_row[p.K]) * total, 0.0);
+  // ---- the drawn token: the CTA that has the warp whose interval holds the target cuts that interval anew, a part to each warp ----
+  const double aim = fmax(u_last * total, 0.0);
   long long* out = p.tokens + static_cast<size_t>(b) * (p.K + 1);
-  if (before <= aim && aim < behind) {
-    double run = before;
-    int pick = -1, kept = -1;
-    for (int j0 = lo; j0 < hi && pick < 0; j0 += 32) {
-      const double w = j0 + lane < hi ? weight(j0 + lane) : 0.0;
-      double incl = w;
+  if (lane == 0 && before <= aim && aim < behind) { s_run = lo; s_before = before; }
+  __syncthreads();
+  if (s_run >= 0) {
+    const int run_lo = s_run, run_hi = min(p.V, run_lo + per_warp);
+    const int part = (per_warp / kVerifyWarps + N - 1) / N * N;   // (per_warp is at least 32 N, twice the warps)
+    const int a0 = min(run_hi, run_lo + warp * part), a1 = warp == kVerifyWarps - 1 ? run_hi : min(run_hi, a0 + part);
+    int my_last;
+    const double sum = warp_mass<T, N>(weights, a0, a1, my_last);
+    __syncthreads();
+    if (lane == 0) { warp_sums[warp] = sum; warp_last[warp] = my_last; }
+    __syncthreads();
+    double edge = s_before;
+    int chosen = -1, fallback = -1;
+    double from = 0.0;
 #pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const double v = __shfl_up_sync(0xffffffffu, incl, o);
-        if (lane >= o) incl += v;
-      }
-      const uint32_t hit = __ballot_sync(0xffffffffu, w > 0.0 && run + incl > aim), some = __ballot_sync(0xffffffffu, w > 0.0);
-      if (hit) pick = j0 + __ffs(hit) - 1;
-      if (some) kept = j0 + 31 - __clz(some);
-      run += __shfl_sync(0xffffffffu, incl, 31);
+    for (int w = 0; w < kVerifyWarps; ++w) {
+      const double next = edge + warp_sums[w];
+      if (chosen < 0 && aim < next) { chosen = w; from = edge; }
+      if (warp_last[w] >= 0) fallback = w;
+      edge = next;
     }
-    if (lane == 0) out[n] = pick >= 0 ? pick : kept;   // (the walk's own rounding at the interval's end: the last with a weight)
+    if (chosen < 0) {   // the new sums are a rounding shorter: the last token with a weight
+      if (threadIdx.x == 0) out[n] = warp_last[fallback < 0 ? 0 : fallback];
+    } else if (warp == chosen) {
+      double run = from;
+      int pick = -1, kept = -1;
+      for (int j0 = a0; j0 < a1 && pick < 0; j0 += 32) {
+        double w[1] = {0.0};
+        if (j0 + lane < a1) weights(j0 + lane, w);
+        double incl = w[0];
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const double v = __shfl_up_sync(0xffffffffu, incl, o);
+          if (lane >= o) incl += v;
+        }
+        const uint32_t hit = __ballot_sync(0xffffffffu, w[0] > 0.0 && run + incl > aim), some = __ballot_sync(0xffffffffu, w[0] > 0.0);
+        if (hit) pick = j0 + __ffs(hit) - 1;
+        if (some) kept = j0 + 31 - __clz(some);
+        run += __shfl_sync(0xffffffffu, incl, 31);
+      }
+      if (lane == 0) out[n] = pick >= 0 ? pick : kept;   // (the walk's own rounding at the end: the last with a weight)
+    }
   }
   if (crank == 0) {
     if (threadIdx.x == 0) {
@@ -185,11 +277,11 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_drafts_kernel(const Ver
   }
 }
 
-template <typename T>
+template <typename T, int N>
 static int launch_verify(const VerifyParams& p, int B, cudaStream_t s) {
   // CTAs per sequence: enough of them to keep the memory busy
   const int ctas = B <= 18 ? 16 : B <= 37 ? 8 : B <= 148 ? 4 : 2;
-  auto kernel = verify_drafts_kernel<T>;
+  auto kernel = verify_drafts_kernel<T, N>;
   static bool configured[64] = {false};
   int dev = 0;
   B200_CHECK_CUDA(cudaGetDevice(&dev));
@@ -229,5 +321,9 @@ B200_API int b200_verify_drafts(const long long* drafts, const void* target, lon
   p.drafts = drafts; p.target = target; p.draft = draft; p.uniform = uniform; p.lens = lens; p.t_b = t_b; p.t_k = t_k; p.d_b = d_b; p.d_k = d_k;
   p.K = K; p.V = V; p.accepted = accepted; p.tokens = tokens;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  B200_DISPATCH_FLOAT(dtype, return launch_verify<T>(p, B, s););
+  // rows that all start on 16 bytes are read 16 bytes at a time
+  const long long size = dtype_size(dtype);
+  const bool wide = (reinterpret_cast<uintptr_t>(target) | reinterpret_cast<uintptr_t>(draft) | static_cast<uintptr_t>(t_b * size) |
+                     static_cast<uintptr_t>(t_k * size) | (draft ? static_cast<uintptr_t>(d_b * size) | static_cast<uintptr_t>(d_k * size) : 0)) % 16 == 0;
+  B200_DISPATCH_FLOAT(dtype, if (wide) return launch_verify<T, 16 / sizeof(T)>(p, B, s); return launch_verify<T, 1>(p, B, s););
 }

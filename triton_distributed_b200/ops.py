@@ -989,12 +989,13 @@ def choose_prefix_splits(batch: int, tokens: int, heads: int, kv_heads: int, sha
     waves times steps of 128 keys, where a CTA's start and end cost about three steps."""
     group = heads // kv_heads
     rows = batch * tokens * group
-    own_ctas = batch * kv_heads * -(-tokens * group // (32 if tokens * group > 16 else 16))
+    blocks = lambda n: -(-n // (8 if n <= 8 else 16 if n <= 16 else 32))  # noqa: E731  (CTAs for n rows of the warp kernel)
+    own_ctas = batch * kv_heads * blocks(tokens * group)
     able = shared > 0 and group <= 128 and page >= 8 and (page % 128 == 0 or 128 % page == 0) and slots < 0x7fffff00 and kv_heads <= 65535
     if variant == "tc" and not able:
         raise ValueError("shared_prefix_attention: these heads or pages are not for the tensor-core kernel")
     tc = able and (rows > 32 if variant is None else variant == "tc")
-    prefix_ctas = kv_heads * -(-rows // (32 if rows > 16 else 16)) if shared and not tc else 0
+    prefix_ctas = kv_heads * blocks(rows) if shared and not tc else 0
     share = max(128, (prefix_ctas * shared + own_ctas * own) // (2 * sm_count))
     chunk = -(-share // 64) * 64
     own_splits = max(1, min(64, -(-own // chunk)))
