@@ -971,22 +971,55 @@ def prefill_attention_vt(q: torch.Tensor, k: torch.Tensor, vt: torch.Tensor, cu_
 
 
 # ---- several continuations of one prompt (csrc/kernels/shared_prefix.cu, verify.cu, pages.cu) --
-def _check_device(name: str, *tensors: torch.Tensor | None) -> None:
-    """All tensors on the current CUDA device: the kernels are launched on its current stream."""
+def _check_device(name: str, *tensors: torch.Tensor | None) -> int:
+    """All tensors on the current CUDA device (whose index is returned): the kernels are launched on its current stream."""
     _lib.require_cuda()
     current = torch.cuda.current_device()
     for t in tensors:
-        if t is not None and (not t.is_cuda or t.device.index != current):
+        if t is not None and t.get_device() != current:
             raise ValueError(f"{name}: all tensors must be on the current CUDA device (cuda:{current}), got {t.device}")
+    return current
+
+
+_P, _I, _L = ctypes.c_void_p, ctypes.c_int, ctypes.c_longlong
+# what the entry points of this section take: with these known, plain numbers are passed without an object for each
+_SERVING_ARGS = {
+    "b200_shared_prefix_attention": (_P, _L, _P, _P, _P, _P, _I, _I, _P, _I, _I, _I, _I, _I, _I, _I, _I, c_float, _I, _I, _I, _P, _P, _P, _P, _I, _P, _P),
+    "b200_verify_drafts": (_P, _P, _L, _L, _P, _L, _L, _P, _P, _I, _I, _I, _P, _P, _I, _P),
+    "b200_fork_pages": (_P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _P, _P),
+    "b200_trim_pages": (_P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _P),
+    "b200_reserve_pages": (_P, _P, _P, _P, _I, _I, _I, _I, _I, _P, _I, _P, _P, _P),
+    "b200_compact_pages": (_P, _P, _P, _P, _I, _I, _I, _I, _P, _I, _P, _P),
+    "b200_copy_pages": (_P, _I, _P, _I, _I, _P),
+}
+_serving_fns: dict = {}
+
+
+def _launch(name: str, launches: int, device: int, *args) -> None:
+    """Call an entry point of ``_SERVING_ARGS`` (None: a null pointer) with the current stream of `device` as its last argument."""
+    fn = _serving_fns.get(name)
+    if fn is None:
+        fn = getattr(_lib.load(), name)
+        fn.argtypes = _SERVING_ARGS[name]
+        _serving_fns[name] = fn
+    stream = torch._C._cuda_getCurrentRawStream(device)
+    if _lib._NVTX:
+        _lib.call(name, *args, stream)
+    else:
+        code = fn(*args, stream)
+        if code:
+            _lib.check(name, code)
+    _count(launches)
 
 
 @functools.lru_cache(maxsize=1024)
 def choose_prefix_splits(batch: int, tokens: int, heads: int, kv_heads: int, shared: int, own: int, page: int = 64, slots: int = 0,
-                         sm_count: int = 148, variant: str | None = None) -> tuple[bool, int, int]:
+                         dim: int = 128, sm_count: int = 148, variant: str | None = None) -> tuple[bool, int, int]:
     """(tensor-core kernel for the shared keys, ranges of the shared keys, ranges of everybody's own keys) for `shared_prefix_attention`.
 
     Warp kernel: one wave of two CTAs per SM, all with about as many keys, at least 128. Tensor-core kernel: the number of ranges with the least
-    waves times steps of 128 keys, where a CTA's start and end cost about three steps."""
+    estimated time, from what a step of 128 keys, a CTA's start and end (6 us) and the partial results of one more range (written and read at 3 TB/s)
+    take; own keys are split only while that leaves SMs without work."""
     group = heads // kv_heads
     rows = batch * tokens * group
     blocks = lambda n: -(-n // (8 if n <= 8 else 16 if n <= 16 else 32))  # noqa: E731  (CTAs for n rows of the warp kernel)
@@ -995,15 +1028,18 @@ def choose_prefix_splits(batch: int, tokens: int, heads: int, kv_heads: int, sha
     if variant == "tc" and not able:
         raise ValueError("shared_prefix_attention: these heads or pages are not for the tensor-core kernel")
     tc = able and (rows > 32 if variant is None else variant == "tc")
-    prefix_ctas = kv_heads * blocks(rows) if shared and not tc else 0
-    share = max(128, (prefix_ctas * shared + own_ctas * own) // (2 * sm_count))
-    chunk = -(-share // 64) * 64
-    own_splits = max(1, min(64, -(-own // chunk)))
     if not tc:
-        return False, min(64, -(-shared // chunk)) if shared else 0, own_splits
+        prefix_ctas = kv_heads * blocks(rows) if shared else 0
+        share = max(128, (prefix_ctas * shared + own_ctas * own) // (2 * sm_count))
+        chunk = -(-share // 64) * 64
+        return False, min(64, -(-shared // chunk)) if shared else 0, max(1, min(64, -(-own // chunk)))
+    own_splits = 1
+    while own_splits < 64 and own_ctas * own_splits < sm_count // 2 and own > 256 * own_splits:
+        own_splits += 1
     tiles = -(-batch * tokens // (128 // group))
     units, steps = kv_heads * -(-tiles // 2), -(-shared // 128)
-    best = min((-(-units * r // sm_count) * (-(-steps // r) + 3), r) for r in range(1, min(steps, 64) + 1))[1]
+    step_us, merge_us = (1.1 if tiles == 1 else 2.2) * dim / 128, (2 if tiles == 1 else 1) * batch * tokens * heads * dim * 8 / 3e6
+    best = min((-(-units * r // sm_count) * (-(-steps // r) * step_us + 6) + r * merge_us, r) for r in range(1, min(steps, 64) + 1))[1]
     return True, best * (2 if tiles == 1 else 1), own_splits
 
 
@@ -1022,48 +1058,51 @@ def shared_prefix_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: tor
     that 128 is a multiple of, or that are multiples of 128); None picks by the rows per KV head. Returns [B * tokens, Hq, D] (and the natural-log LSE fp32 [B * tokens, Hq])."""
     if q.dim() != 3 or k_cache.dim() != 4 or k_cache.shape != v_cache.shape or kv_lens.dim() != 1 or block_table.dim() != 2:
         raise ValueError("shared_prefix_attention: q [B * tokens, Hq, D], caches [num_blocks, page, Hkv, D], kv_lens [B], block_table [B, max_blocks]")
+    shared, tokens = int(shared), int(tokens)
     T, Hq, D = q.shape
     N, page, Hkv, Dk = k_cache.shape
     B, width = block_table.shape
-    shared, tokens = int(shared), int(tokens)
-    if q.dtype not in (torch.bfloat16, torch.float16) or k_cache.dtype != q.dtype or v_cache.dtype != q.dtype:
+    ldt, per_column = block_table.stride()
+    ldq, per_head, per_element = q.stride()
+    dtype = q.dtype
+    at_q, at_k, at_v = q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr()
+    if dtype not in (torch.bfloat16, torch.float16) or k_cache.dtype != dtype or v_cache.dtype != dtype:
         raise TypeError("shared_prefix_attention handles bf16 / f16 (q and caches of one type)")
     if variant not in (None, "tc", "warp"):
         raise ValueError(f"shared_prefix_attention: variant {variant!r}")
     if D not in (64, 128) or Dk != D:
         raise ValueError(f"shared_prefix_attention: head sizes 64 and 128, got {D} and {Dk}")
-    if tokens < 1 or T != B * tokens or kv_lens.shape[0] != B or Hkv < 1 or Hq % Hkv or Hq < 1 or N < 1 or page < 1:
+    if tokens < 1 or T != B * tokens or kv_lens.shape[0] != B or Hkv < 1 or Hq < 1 or Hq % Hkv or N < 1 or page < 1:
         raise ValueError("shared_prefix_attention: the batch, token or head counts do not fit together")
     if kv_lens.dtype != torch.int32 or block_table.dtype != torch.int32 or (prefix_table is not None and prefix_table.dtype != torch.int32):
         raise TypeError("shared_prefix_attention: kv_lens and the tables are int32")
-    if not (k_cache.is_contiguous() and v_cache.is_contiguous() and kv_lens.is_contiguous()) or (width > 1 and block_table.stride(1) != 1):
+    if not (k_cache.is_contiguous() and v_cache.is_contiguous() and kv_lens.is_contiguous()) or (width > 1 and per_column != 1):
         raise ValueError("shared_prefix_attention needs contiguous caches and lengths and a row-major block table")
-    if q.stride(2) != 1 or (Hq > 1 and q.stride(1) != D) or (T > 1 and (q.stride(0) % 8 or q.stride(0) < 0)) or (q.data_ptr() | k_cache.data_ptr() | v_cache.data_ptr()) % 16:
+    if T <= 1:
+        ldq = Hq * D
+    if per_element != 1 or (Hq > 1 and per_head != D) or ldq % 8 or ldq < 0 or (at_q | at_k | at_v) % 16:
         raise ValueError("shared_prefix_attention: q holds whole rows of heads, a multiple of 8 elements apart; q and caches start on 16 bytes")
     blocks = -(-shared // page)
     if shared < 0 or (shared > 0 and prefix_table is None and (width < blocks or B == 0)):
         raise ValueError(f"shared_prefix_attention: {shared} shared keys do not fit the block table")
-    if prefix_table is None:
-        prefix_table = block_table
-    elif prefix_table.dim() != 1 or prefix_table.shape[0] < blocks or not prefix_table.is_contiguous():
+    if prefix_table is not None and (prefix_table.dim() != 1 or prefix_table.shape[0] < blocks or not prefix_table.is_contiguous()):
         raise ValueError("shared_prefix_attention: the prefix table holds the pages of the shared keys")
-    if out is not None and (out.shape != q.shape or out.dtype != q.dtype or not out.is_contiguous()):
+    if out is not None and (out.shape != q.shape or out.dtype != dtype or not out.is_contiguous()):
         raise ValueError("shared_prefix_attention: the output is contiguous and has the shape and type of q")
-    _check_device("shared_prefix_attention", q, k_cache, v_cache, kv_lens, block_table, prefix_table, out)
+    device = _check_device("shared_prefix_attention", q, k_cache, v_cache, kv_lens, block_table, prefix_table, out)
     if out is None:
-        out = torch.empty((T, Hq, D), dtype=q.dtype, device=q.device)
-    lse = torch.empty((T, Hq), dtype=torch.float32, device=q.device) if return_lse else None
+        out = q.new_empty((T, Hq, D))
+    lse = q.new_empty((T, Hq), dtype=torch.float32) if return_lse else None
     if B:
         longest = width * page if max_kv_len is None else min(int(max_kv_len), width * page)
-        tc, prefix_splits, own_splits = choose_prefix_splits(B, tokens, Hq, Hkv, shared, max(1, longest - shared), page, N * page, variant=variant)
+        tc, prefix_splits, own_splits = choose_prefix_splits(B, tokens, Hq, Hkv, shared, max(1, longest - shared), page, N * page, D, variant=variant)
         ranges = T * Hq * (prefix_splits + own_splits)
-        part = torch.empty(ranges * (D + 1), dtype=torch.float32, device=q.device)   # outputs of all ranges, then their log-sum-exps
+        part = q.new_empty(ranges * (D + 1), dtype=torch.float32)   # outputs of all ranges, then their log-sum-exps
         at = part.data_ptr()
-        _lib.call("b200_shared_prefix_attention", ptr(q), ctypes.c_longlong(q.stride(0) if T > 1 else Hq * D), ptr(k_cache), ptr(v_cache), ptr(kv_lens),
-                  ptr(block_table), block_table.stride(0), width, ptr(prefix_table), B, tokens, Hq, Hkv, D, N, page, shared, c_float(scale),
-                  int(tc), prefix_splits, own_splits, ctypes.c_void_p(at), ctypes.c_void_p(at + ranges * D * 4), ptr(out), ptr(lse), dtype_code(q.dtype),
-                  ptr(_pipeline_status(q.device)), stream_ptr())
-        _count(3 if tc else 2)
+        table = block_table.data_ptr()
+        _launch("b200_shared_prefix_attention", 3 if tc else 2, device, at_q, ldq, at_k, at_v, kv_lens.data_ptr(), table, ldt, width,
+                table if prefix_table is None else prefix_table.data_ptr(), B, tokens, Hq, Hkv, D, N, page, shared, scale, tc, prefix_splits, own_splits, at,
+                at + ranges * D * 4, out.data_ptr(), _dptr(lse), dtype_code(dtype), _pipeline_status(q.device).data_ptr())
     return (out, lse) if return_lse else out
 
 
@@ -1083,69 +1122,69 @@ def verify_drafts(drafts: torch.Tensor, target_probs: torch.Tensor, uniform: tor
         raise ValueError("verify_drafts: drafts [B, K], target_probs [B, K + 1, V]")
     B, K = drafts.shape
     V = target_probs.shape[2]
-    if target_probs.shape[:2] != (B, K + 1) or V < 1 or uniform.shape != (B, K + 1) or (draft_probs is not None and draft_probs.shape != (B, K, V)) \
+    if target_probs.shape != (B, K + 1, V) or V < 1 or uniform.shape != (B, K + 1) or (draft_probs is not None and draft_probs.shape != (B, K, V)) \
             or (draft_lens is not None and draft_lens.shape != (B,)):
         raise ValueError("verify_drafts: target_probs [B, K + 1, V], uniform [B, K + 1], draft_probs [B, K, V], draft_lens [B]")
+    dtype = target_probs.dtype
     if drafts.dtype != torch.int64 or uniform.dtype != torch.float32 or (draft_lens is not None and draft_lens.dtype != torch.int32):
         raise TypeError("verify_drafts: drafts int64, uniform fp32, draft_lens int32")
-    if target_probs.dtype not in (torch.float32, torch.bfloat16, torch.float16) or (draft_probs is not None and draft_probs.dtype != target_probs.dtype):
+    if dtype not in (torch.float32, torch.bfloat16, torch.float16) or (draft_probs is not None and draft_probs.dtype != dtype):
         raise TypeError("verify_drafts: probabilities of one type, fp32, bf16 or f16")
-    if (V > 1 and (target_probs.stride(2) != 1 or (draft_probs is not None and K > 0 and draft_probs.stride(2) != 1))) or not drafts.is_contiguous() \
-            or not uniform.is_contiguous() or (draft_lens is not None and not draft_lens.is_contiguous()):
+    t_b, t_k, t_v = target_probs.stride()
+    d_b, d_k, d_v = draft_probs.stride() if draft_probs is not None else (0, 0, 1)
+    if (V > 1 and (t_v != 1 or (K > 0 and d_v != 1))) or not drafts.is_contiguous() or not uniform.is_contiguous() \
+            or (draft_lens is not None and not draft_lens.is_contiguous()):
         raise ValueError("verify_drafts: probabilities with unit stride along the vocabulary, the rest contiguous")
-    _check_device("verify_drafts", drafts, target_probs, uniform, draft_probs, draft_lens)
-    accepted = torch.empty(B, dtype=torch.int32, device=drafts.device)
-    tokens = torch.empty((B, K + 1), dtype=torch.int64, device=drafts.device)
-    ll = ctypes.c_longlong
-    d_b, d_k = (draft_probs.stride(0), draft_probs.stride(1)) if draft_probs is not None else (0, 0)
+    device = _check_device("verify_drafts", drafts, target_probs, uniform, draft_probs, draft_lens)
+    accepted, tokens = drafts.new_empty(B, dtype=torch.int32), drafts.new_empty((B, K + 1))
     if B:
-        _lib.call("b200_verify_drafts", ptr(drafts), ptr(target_probs), ll(target_probs.stride(0)), ll(target_probs.stride(1)), ptr(draft_probs), ll(d_b),
-                  ll(d_k), ptr(uniform), ptr(draft_lens), B, K, V, ptr(accepted), ptr(tokens), dtype_code(target_probs.dtype), stream_ptr())
-        _count()
+        _launch("b200_verify_drafts", 1, device, drafts.data_ptr(), target_probs.data_ptr(), t_b, t_k, _dptr(draft_probs), d_b, d_k, uniform.data_ptr(),
+                _dptr(draft_lens), B, K, V, accepted.data_ptr(), tokens.data_ptr(), dtype_code(dtype))
     return accepted, tokens
 
 
-class _PageTensor(ctypes.Structure):
-    """Mirror of ``b200::PageTensor`` (csrc/kernels/pages.cu)."""
-    _fields_ = [("base", ctypes.c_void_p), ("layers", ctypes.c_longlong), ("layer_stride", ctypes.c_longlong), ("page_bytes", ctypes.c_longlong),
-                ("row_bytes", ctypes.c_longlong)]
-
-
 def _page_tensors(name: str, caches, dim: int, pages: int | None = None):
-    """(native descriptions, tokens per page) of tensors whose dimension `dim` (0, or 1 behind layers) counts pages."""
-    caches = list(caches)
+    """(caches, descriptions, tokens per page) of tensors whose dimension `dim` (0, or 1 behind layers) counts pages. A description is a
+    ``b200::PageTensor`` (csrc/kernels/pages.cu): address, layers, bytes from a layer, a page and a token's row to the next."""
     if dim not in (0, 1):
         raise ValueError(f"{name}: pages are counted by dimension 0, or 1 behind the layers")
-    page, out = None, (_PageTensor * max(1, len(caches)))()
-    for i, t in enumerate(caches):
-        if t.dim() < dim + 2 or (pages is not None and t.shape[dim] < pages) or t.numel() == 0:
+    caches = tuple(caches)
+    page, fields = None, []
+    for t in caches:
+        shape, strides, size = t.shape, t.stride(), t.element_size()
+        if len(shape) < dim + 2 or (pages is not None and shape[dim] < pages) or t.numel() == 0:
             raise ValueError(f"{name}: a cache is [{'layers, ' if dim else ''}pages, tokens, ...] with as many pages as the counts have")
-        if page is not None and t.shape[dim + 1] != page:
+        if page is not None and shape[dim + 1] != page:
             raise ValueError(f"{name}: the caches differ in the tokens of a page")
-        page = t.shape[dim + 1]
-        one = t[0] if dim else t
-        if not one.is_contiguous():
+        page = shape[dim + 1]
+        if not t.is_contiguous() and not (dim and t[0].is_contiguous()):
             raise ValueError(f"{name}: the pages of a layer must be contiguous")
-        size, row = t.element_size(), one[0, 0].numel()
-        out[i] = _PageTensor(t.data_ptr(), t.shape[0] if dim else 1, t.stride(0) * size if dim else 0, page * row * size, row * size)
-    return caches, out, page
+        row = 1
+        for n in shape[dim + 2:]:
+            row *= n
+        fields += t.data_ptr(), shape[0] if dim else 1, strides[0] * size if dim else 0, page * row * size, row * size
+    return caches, (_L * len(fields))(*fields), page
 
 
 def _check_page_state(name: str, block_table, refs, kv_lens=None, page=1) -> tuple[int, int, int]:
     if block_table.dim() != 2 or refs.dim() != 1 or not block_table.numel() or not refs.numel() or (kv_lens is not None and kv_lens.shape != block_table.shape[:1]):
         raise ValueError(f"{name}: block_table [rows, max_blocks], kv_lens [rows], refs [pages]")
-    if any(t is not None and (t.dtype != torch.int32 or not t.is_contiguous()) for t in (block_table, refs, kv_lens)):
-        raise TypeError(f"{name}: the block table, the lengths and the counts are contiguous int32")
+    for t in (block_table, refs, kv_lens):
+        if t is not None and (t.dtype != torch.int32 or not t.is_contiguous()):
+            raise TypeError(f"{name}: the block table, the lengths and the counts are contiguous int32")
     if page < 1:
         raise ValueError(f"{name}: a page holds at least one token")
-    return block_table.shape[0], block_table.shape[1], refs.shape[0]
+    return *block_table.shape, refs.shape[0]
 
 
 def _rows(name: str, rows, device) -> torch.Tensor:
-    t = torch.as_tensor(rows, device=device)
-    if t.dim() != 1 or (t.dtype not in (torch.int32, torch.int64) and t.numel()):
+    if not isinstance(rows, torch.Tensor):
+        rows = torch.as_tensor(rows, device=device)
+    if rows.dim() != 1 or (rows.dtype not in (torch.int32, torch.int64) and rows.numel()):
         raise ValueError(f"{name}: rows are a list or a 1-D tensor of whole numbers")
-    return t.to(torch.int32).contiguous()
+    if rows.dtype == torch.int32 and rows.is_contiguous() and rows.device == device:
+        return rows
+    return rows.to(device=device, dtype=torch.int32).contiguous()
 
 
 def fork_pages(block_table: torch.Tensor, kv_lens: torch.Tensor, refs: torch.Tensor, src, dst, page_size: int) -> None:
@@ -1157,12 +1196,12 @@ def fork_pages(block_table: torch.Tensor, kv_lens: torch.Tensor, refs: torch.Ten
     src, dst = _rows("fork_pages", src, block_table.device), _rows("fork_pages", dst, block_table.device)
     if src.shape != dst.shape:
         raise ValueError("fork_pages: as many sources as destinations")
-    _check_device("fork_pages", block_table, kv_lens, refs, src, dst)
+    device = _check_device("fork_pages", block_table, kv_lens, refs, src, dst)
     n = src.shape[0]
     if n:
-        scratch = torch.empty(n * (W + 1), dtype=torch.int32, device=block_table.device)
-        _lib.call("b200_fork_pages", ptr(block_table), ptr(kv_lens), ptr(refs), ptr(src), ptr(dst), n, R, W, N, int(page_size), ptr(scratch), stream_ptr())
-        _count(2)
+        scratch = refs.new_empty(n * (W + 1))
+        _launch("b200_fork_pages", 2, device, block_table.data_ptr(), kv_lens.data_ptr(), refs.data_ptr(), src.data_ptr(), dst.data_ptr(), n, R, W, N, page_size,
+                scratch.data_ptr())
 
 
 def trim_pages(block_table: torch.Tensor, kv_lens: torch.Tensor, refs: torch.Tensor, page_size: int, lens: torch.Tensor | None = None, rows=None) -> None:
@@ -1173,10 +1212,9 @@ def trim_pages(block_table: torch.Tensor, kv_lens: torch.Tensor, refs: torch.Ten
     n = R if rows is None else rows.shape[0]
     if lens is not None and (lens.dtype != torch.int32 or lens.shape != (n,) or not lens.is_contiguous()):
         raise ValueError("trim_pages: one length (int32) for every row")
-    _check_device("trim_pages", block_table, kv_lens, refs, rows, lens)
+    device = _check_device("trim_pages", block_table, kv_lens, refs, rows, lens)
     if n:
-        _lib.call("b200_trim_pages", ptr(block_table), ptr(kv_lens), ptr(refs), ptr(rows), ptr(lens), n, R, W, N, int(page_size), stream_ptr())
-        _count()
+        _launch("b200_trim_pages", 1, device, block_table.data_ptr(), kv_lens.data_ptr(), refs.data_ptr(), _dptr(rows), _dptr(lens), n, R, W, N, page_size)
 
 
 def reserve_pages(block_table: torch.Tensor, kv_lens: torch.Tensor, refs: torch.Tensor, count, caches, dim: int = 0,
@@ -1201,13 +1239,12 @@ def reserve_pages(block_table: torch.Tensor, kv_lens: torch.Tensor, refs: torch.
         raise ValueError("reserve_pages: the count of tokens is not negative")
     if status is not None and (status.dtype != torch.int32 or status.numel() != 1):
         raise ValueError("reserve_pages: the status is one int32")
-    _check_device("reserve_pages", block_table, kv_lens, refs, counts, status, *caches)
+    device = _check_device("reserve_pages", block_table, kv_lens, refs, counts, status, *caches)
     if status is None:
-        status = torch.empty(1, dtype=torch.int32, device=refs.device)
-    scratch = torch.empty(8 * (R + N) + 16, dtype=torch.int32, device=refs.device)   # b200_pages_scratch
-    _lib.call("b200_reserve_pages", ptr(block_table), ptr(kv_lens), ptr(refs), ptr(counts), int(count), R, W, N, page, tensors, len(caches), ptr(scratch),
-              ptr(status), stream_ptr())
-    _count(2)
+        status = refs.new_empty(1)
+    scratch = refs.new_empty(8 * (R + N) + 16)   # b200_pages_scratch
+    _launch("b200_reserve_pages", 2, device, block_table.data_ptr(), kv_lens.data_ptr(), refs.data_ptr(), _dptr(counts), count, R, W, N, page, tensors, len(caches),
+            scratch.data_ptr(), status.data_ptr())
     return status
 
 
@@ -1221,10 +1258,10 @@ def compact_pages(block_table: torch.Tensor, refs: torch.Tensor, caches, dim: in
         out = torch.empty_like(block_table), torch.empty_like(refs)
     elif out[0].shape != block_table.shape or out[1].shape != refs.shape or any(t.dtype != torch.int32 or not t.is_contiguous() for t in out):
         raise ValueError("compact_pages: the new tables are laid out like the old ones")
-    _check_device("compact_pages", block_table, refs, *out, *caches)
-    scratch = torch.empty(8 * (R + N) + 16, dtype=torch.int32, device=refs.device)
-    _lib.call("b200_compact_pages", ptr(block_table), ptr(out[0]), ptr(refs), ptr(out[1]), R, W, N, page or 1, tensors, len(caches), ptr(scratch), stream_ptr())
-    _count(2)
+    device = _check_device("compact_pages", block_table, refs, *out, *caches)
+    scratch = refs.new_empty(8 * (R + N) + 16)   # b200_pages_scratch
+    _launch("b200_compact_pages", 2, device, block_table.data_ptr(), out[0].data_ptr(), refs.data_ptr(), out[1].data_ptr(), R, W, N, page or 1, tensors, len(caches),
+            scratch.data_ptr())
     return out
 
 
@@ -1241,8 +1278,7 @@ def copy_pages(caches, src: list[int], dst: list[int], dim: int = 0, tokens: lis
         raise ValueError("copy_pages: a page or a count of tokens is out of range")
     if len(set(dst)) != len(dst) or set(dst) & set(src):
         raise ValueError("copy_pages: a page is the destination of several copies, or of one and the source of another")
-    _check_device("copy_pages", *caches)
+    device = _check_device("copy_pages", *caches)
     if src:
         moves = torch.tensor([[s, d, n, 0] for s, d, n in zip(src, dst, tokens)], dtype=torch.int32).to(caches[0].device)
-        _lib.call("b200_copy_pages", tensors, len(caches), ptr(moves), len(src), N, stream_ptr())
-        _count()
+        _launch("b200_copy_pages", 1, device, tensors, len(caches), moves.data_ptr(), len(src), N)
