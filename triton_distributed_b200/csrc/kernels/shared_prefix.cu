@@ -436,8 +436,8 @@ using namespace b200;
 // q [B * T, Hq, D] with ldq elements between tokens; caches [num_blocks, page, Hkv, D] contiguous; kv_lens int32 [B]; block_table int32
 // [B, width] with bt_stride between rows; prefix_table int32 [>= ceil(shared / page)]; o_part fp32 [B * T * Hq, prefix_splits +
 // own_splits, D] and lse_part fp32 [B * T * Hq, prefix_splits + own_splits] are scratch; out [B * T, Hq, D] contiguous, out_lse nullable
-// fp32 [B * T, Hq]. 16-byte aligned q, caches, out. tc: the shared keys go to the tensor-core kernel (an even number of ranges where all rows
-// of a KV head fit one tile of floor(128 / (Hq / Hkv)) tokens). With shared = 0: tc = 0, prefix_splits = 0.
+// fp32 [B * T, Hq]. 16-byte aligned q, caches, out. tc: the shared keys go to the tensor-core kernel. With shared = 0:
+// tc = 0, prefix_splits = 0.
 B200_API int b200_shared_prefix_attention(const void* q, long long ldq, const void* k_cache, const void* v_cache, const int* kv_lens, const int* block_table,
                                           int bt_stride, int width, const int* prefix_table, int B, int T, int Hq, int Hkv, int D, int num_blocks,
                                           int page, int shared, float scale, int tc, int prefix_splits, int own_splits, float* o_part, float* lse_part, void* out,
@@ -463,10 +463,7 @@ B200_API int b200_shared_prefix_attention(const void* q, long long ldq, const vo
   long long ctas = 0;
   if (tc) {
     B200_REQUIRE(shared_prefix_tc_takes(p, D), "shared-prefix attention: these heads or pages are not for the tensor-core kernel");
-    const bool two_ranges = static_cast<long long>(B) * T <= 128 / G;
-    B200_REQUIRE(!two_ranges || prefix_splits % 2 == 0, "shared-prefix attention: rows of one tile take pairs of ranges");
-    const int per_row = two_ranges ? prefix_splits / 2 : prefix_splits;
-    p.prefix_chunk = ((shared + per_row - 1) / per_row + 127) / 128 * 128;
+    p.prefix_chunk = ((shared + prefix_splits - 1) / prefix_splits + 127) / 128 * 128;
     const int rc = shared_prefix_tc_launch(p, D, dtype, s);
     if (rc != kOk) return rc;
     p.late_wait = pdl_enabled();

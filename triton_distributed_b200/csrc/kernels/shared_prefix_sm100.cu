@@ -9,14 +9,18 @@
 // ping-pong scheduling, FlashAttention-3, Shah et al. 2024):
 //   warps 0-3    softmax of tile 0, one thread per row
 //   warps 4-7    softmax of tile 1
-//   warps 8-11   rescale the output of either tile when a row has a new maximum
-//   warp 12      TMA producer: the query tiles, then K and V tiles page by page through their rings (128-byte swizzle)
-//   warp 13      one elected thread issues tcgen05.mma, for each step and tile O += P V of this step, then S = Q K^T of the next
+//   warp 8       TMA producer: the query tiles, then K and V tiles page by page through their rings (128-byte swizzle)
+//   warp 9       one elected thread issues tcgen05.mma, for each step and tile O += P V of this step, then S = Q K^T of the next
 // Tensor memory: S of tile t at columns 128 t, O of tile t at 256 + 128 t. P is written over S as 16-bit pairs and is the A operand of
-// the second product; V is read in place as an MN-major B operand. The reference of a row's softmax is its running maximum itself.
+// the second product; V is read in place as an MN-major B operand.
+// The softmax of a step does not wait for its maximum: the weights are taken against the reference of the steps before, and only if one of
+// a warp's comes out above 2^8 (or at the first step) the warp raises its rows' references to their maxima, rescales their output and takes the step's
+// weights anew from the scores, which are still there because the weights stay in registers until then. Over a long range the maximum of the first
+// steps stands, so this is rare, and the chain of a step is one pass over the scores instead of two. Weights above one are rounded like those
+// below (relative to themselves); what is lost is that a row's largest weight was held exactly: error against 64 bits 2.3e-3 of the norm before and now.
 // Pages: a step's 128 keys are 128 / page copies (or one, of pages of 128 and more); page numbers are read a window of 32 ahead by
 // the producer's lanes. Pages outside the cache are copies from behind its end, which give zeros.
-// Rows leave their normalised output in fp32 and their log-sum-exp, one range per CTA (two with kTwoRanges).
+// Rows leave their normalised output in fp32 and their log-sum-exp, one range per CTA.
 #include "b200/host.h"
 #include "b200/packed_f32.cuh"
 #include "b200/primitives.cuh"
@@ -27,14 +31,15 @@ namespace b200 {
 
 constexpr int kXM = 128, kXN = 128;            // rows per tile, keys per step
 constexpr int kXAtom = 128 * 64 * 2;           // 128 rows x 64 columns of 16 bits: 16 KB
-constexpr int kXThreads = 512;
-constexpr int kXSoftmaxRegs = 184, kXScaleRegs = 72, kXOtherRegs = 72;   // 256 x 184 + 128 x 72 + 128 x 72 = 512 x 128
+constexpr int kXThreads = 384;
+constexpr int kXSoftmaxRegs = 208, kXOtherRegs = 88;   // 256 x 208 + 128 x 88 = 384 x 168, what the block starts with
+constexpr float kXRaise = 256.f;               // a weight above it raises the reference (f16 holds 2^8 times as much)
 template <int kAtoms, bool kTwoRanges>
 struct PrefixShape {
   static constexpr int kTile = kAtoms * kXAtom;
   static constexpr int kQTiles = kTwoRanges ? 1 : 2;
   static constexpr int kStages = kTwoRanges ? (kAtoms == 2 ? 3 : 4) : (kAtoms == 2 ? 2 : 4);   // of K, and as many of V
-  static constexpr int kSmem = kQTiles * kTile + 2 * kStages * kTile + 1024 /*alignment*/ + 512 /*barriers*/ + 2 * kXM * 4 /*factors*/;
+  static constexpr int kSmem = kQTiles * kTile + 2 * kStages * kTile + 1024 /*alignment*/ + 256 /*barriers*/ + kXM * 8 /*maxima and sums of the odd steps*/;
 };
 
 __device__ __forceinline__ float prefix_exp2(float x) {   // one instruction; -inf gives 0
@@ -68,10 +73,9 @@ shared_prefix_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
   uint64_t* s_full = bars + 17;      // [2 tiles] scores are in tensor memory (and the tile's earlier products are done)
   uint64_t* p_full = bars + 19;      // [2 tiles] probabilities are in tensor memory, and the output has been rescaled
   uint64_t* o_full = bars + 21;      // [2 tiles] the last product is done
-  uint64_t* c_full = bars + 23;      // [2 tiles] a step's factors of the output have been written
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 25);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 23);
   volatile uint32_t* abort_flag = tmem_slot + 1;
-  float* s_factor = reinterpret_cast<float*>(bars + 32);   // [2 tiles][128 rows]
+  float2* s_odd = reinterpret_cast<float2*>(bars + 32);    // [128 rows] kTwoRanges: reference and sum of the odd steps
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint64_t timeout_ns = 4000000000ull;
@@ -93,9 +97,8 @@ shared_prefix_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
     }
     for (int t = 0; t < 2; ++t) {
       mbar_init(s_full + t, 1);
-      mbar_init(p_full + t, 8);   // four warps of softmax, four that rescale
+      mbar_init(p_full + t, 4);
       mbar_init(o_full + t, 1);
-      mbar_init(c_full + t, 4);
     }
     *abort_flag = 0;
     mbar_fence_init();
@@ -109,7 +112,7 @@ shared_prefix_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
     *reinterpret_cast<uint4*>(sQ + a * kXAtom + r * 128 + chunk * 16) = make_uint4(0, 0, 0, 0);
   }
   fence_view_async_shared();
-  if (warp == 15) tmem_alloc(tmem_slot, 512);
+  if (warp == 10) tmem_alloc(tmem_slot, 512);
   tc_fence_before_sync();
   __syncthreads();
   tc_fence_after_sync();
@@ -117,9 +120,9 @@ shared_prefix_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
   griddep_wait();
   griddep_launch_dependents();
 
-  if (warp >= 12) {
+  if (warp >= 8) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kXOtherRegs));
-    if (warp == 12) {
+    if (warp == 8) {
       // ---------------------------------------------------------------- TMA producer: the warp reads page numbers, lane 0 copies
       const int rows = min(p.page, kXN), pieces = kXN / rows;   // keys per copy, copies per step
       const int piece0 = key0 / rows, piece_end = (p.shared + rows - 1) / rows;   // copies are numbered from the first key on
@@ -177,7 +180,7 @@ shared_prefix_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
         for (int c = max(0, vc - kSt); c < vc; ++c) mbar_wait(v_full + c % kSt, (c / kSt) & 1, &never, timeout_ns);
       }
       __syncwarp();
-    } else if (warp == 13) {
+    } else if (warp == 9) {
       // ---------------------------------------------------------------- MMA issuer
       if (elect_one()) {
         const uint32_t idesc_s = umma_idesc_f16(kXM, kXN, BF16);
@@ -257,40 +260,6 @@ shared_prefix_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
       }
       __syncwarp();
     }
-  } else if (warp >= 8) {
-    // ------------------------------------------------------------------ rescaling, one thread per row of either tile
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kXScaleRegs));
-    const int row = (warp & 3) * 32 + lane;
-    const uint32_t o_lanes = tmem_base + (static_cast<uint32_t>((warp & 3) * 32) << 16) + 2 * kXN;
-    const int most = max(steps_of(0), steps_of(1));
-    bool ok = true;
-    for (int j = 1; j < most && ok; ++j) {
-      for (int t = 0; t < 2; ++t) {
-        if (j >= steps_of(t)) continue;
-        ok = __all_sync(0xffffffffu, mbar_wait(c_full + t, (j - 1) & 1, abort_flag, timeout_ns));
-        if (!ok) break;
-        tc_fence_after_sync();
-        const float corr = s_factor[t * kXM + row];
-        if (__any_sync(0xffffffffu, corr != 1.f)) {
-          // the scores of this step were issued after the tile's last product, so O is complete and nothing writes it now
-          const uint32_t o_addr = o_lanes + t * 128;
-          uint32_t o[2][16];
-          tmem_ld_32x16(o_addr, o[0]);
-#pragma unroll
-          for (int c = 0; c < D / 16; ++c) {
-            tmem_ld_wait();
-            if (c < D / 16 - 1) tmem_ld_32x16(o_addr + (c + 1) * 16, o[(c + 1) & 1]);
-#pragma unroll
-            for (int e = 0; e < 16; ++e) o[c & 1][e] = __float_as_uint(__uint_as_float(o[c & 1][e]) * corr);
-            tmem_st_32x16(o_addr + c * 16, o[c & 1]);
-          }
-          tmem_st_wait();
-        }
-        tc_fence_before_sync();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(p_full + t);
-      }
-    }
   } else {
     // ------------------------------------------------------------------ softmax, one thread per row
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kXSoftmaxRegs));
@@ -305,54 +274,96 @@ shared_prefix_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
       ok = __all_sync(0xffffffffu, mbar_wait(s_full + t, j & 1, abort_flag, timeout_ns));
       if (!ok) break;
       tc_fence_after_sync();
-      uint32_t r[4][32];
-#pragma unroll
-      for (int c = 0; c < 4; ++c) tmem_ld_32x32(s_addr + c * 32, r[c]);
-      tmem_ld_wait();
       const int visible = key1 - key0 - c_step * kXN;
-      if (visible < kXN) {
-#pragma unroll
-        for (int c = 0; c < 4; ++c)
+      uint32_t packed[4][16];
+      f32x2 sums[2];
+      // scores 32 c ... of the row, those behind the last key at -inf
+      auto fetch = [&](int c, uint32_t (&r)[32]) { tmem_ld_32x32(s_addr + c * 32, r); };
+      auto hide_tail = [&](int c, uint32_t (&r)[32]) {
+        if (visible < (c + 1) * 32) {
 #pragma unroll
           for (int e = 0; e < 32; ++e)
-            if (c * 32 + e >= visible) r[c][e] = __float_as_uint(-INFINITY);
-      }
-      float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-      for (int e = 0; e < 32; ++e)
-#pragma unroll
-        for (int c = 0; c < 4; ++c) mx[c] = fmaxf(mx[c], __uint_as_float(r[c][e]));
-      const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * p.scale_log2e;
-      if (j == 0) {
-        ref = top;
-      } else {
-        // (the factors of the step before have been used: this step's scores were issued behind that step's product)
-        float corr = 1.f;
-        if (top > ref) {
-          corr = prefix_exp2(ref - top);
-          ref = top;
+            if (c * 32 + e >= visible) r[e] = __float_as_uint(-INFINITY);
         }
-        sum *= corr;
-        s_factor[t * kXM + row] = corr;
-        __syncwarp();
-        if (lane == 0) mbar_arrive(c_full + t);
-      }
-      const float base = ref == -INFINITY ? 0.f : ref;
-      const f32x2 scale2 = pack2(p.scale_log2e, p.scale_log2e), base2 = pack2(-base, -base);
-      f32x2 sums[2] = {pack2(0.f, 0.f), pack2(0.f, 0.f)};
-#pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        uint32_t packed[16];
+      };
+      const f32x2 scale2 = pack2(p.scale_log2e, p.scale_log2e);
+      auto weigh = [&](int c, const uint32_t (&r)[32], f32x2 base2) {
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
-          // 2^(s * scale - base): one fused multiply-add for two scores, one special-function instruction each
-          const float2 x = unpack2(fma2(pack2(__uint_as_float(r[c][2 * e]), __uint_as_float(r[c][2 * e + 1])), scale2, base2));
+          // 2^(s * scale - reference): one fused multiply-add for two scores, one special-function instruction each
+          const float2 x = unpack2(fma2(pack2(__uint_as_float(r[2 * e]), __uint_as_float(r[2 * e + 1])), scale2, base2));
           const float p0 = prefix_exp2(x.x), p1 = prefix_exp2(x.y);
           sums[e & 1] = add2(sums[e & 1], pack2(p0, p1));
-          packed[e] = BF16 ? pack_bf16x2(p0, p1) : pack_f16x2(p0, p1);
+          packed[c][e] = BF16 ? pack_bf16x2(p0, p1) : pack_f16x2(p0, p1);
         }
-        tmem_st_32x16(s_addr + c * 16, packed);
+      };
+      bool raise = j == 0;
+      if (j > 0) {
+        sums[0] = sums[1] = pack2(0.f, 0.f);
+        const f32x2 base2 = pack2(-ref, -ref);
+        uint32_t r[2][32];
+        fetch(0, r[0]);
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          tmem_ld_wait();
+          if (c < 3) fetch(c + 1, r[(c + 1) & 1]);
+          hide_tail(c, r[c & 1]);
+          weigh(c, r[c & 1], base2);
+        }
+        float most = 0.f;
+        if (BF16) {
+          __nv_bfloat162 m = *reinterpret_cast<__nv_bfloat162*>(&packed[0][0]);
+#pragma unroll
+          for (int e = 1; e < 64; ++e) m = __hmax2(m, *reinterpret_cast<__nv_bfloat162*>(&packed[e >> 4][e & 15]));
+          most = fmaxf(__low2float(m), __high2float(m));
+        } else {
+          __half2 m = *reinterpret_cast<__half2*>(&packed[0][0]);
+#pragma unroll
+          for (int e = 1; e < 64; ++e) m = __hmax2(m, *reinterpret_cast<__half2*>(&packed[e >> 4][e & 15]));
+          most = fmaxf(__low2float(m), __high2float(m));
+        }
+        raise = __any_sync(0xffffffffu, most > kXRaise || ref == -INFINITY);
       }
+      if (raise) {
+        float mx = -INFINITY;
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          uint32_t r[32];
+          fetch(c, r);
+          tmem_ld_wait();
+          hide_tail(c, r);
+#pragma unroll
+          for (int e = 0; e < 32; ++e) mx = fmaxf(mx, __uint_as_float(r[e]));
+        }
+        const float top = fmaxf(ref, mx * p.scale_log2e), base = top == -INFINITY ? 0.f : top;
+        const float corr = ref == -INFINITY ? 0.f : prefix_exp2(ref - base);
+        ref = top;
+        sum *= corr;
+        if (j > 0) {
+          // the scores of this step were issued after the tile's last product, so O is complete and nothing writes it now
+#pragma unroll
+          for (int c = 0; c < D / 16; ++c) {
+            uint32_t o[16];
+            tmem_ld_32x16(o_addr + c * 16, o);
+            tmem_ld_wait();
+#pragma unroll
+            for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * corr);
+            tmem_st_32x16(o_addr + c * 16, o);
+          }
+        }
+        sums[0] = sums[1] = pack2(0.f, 0.f);
+        const f32x2 base2 = pack2(-base, -base);
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          uint32_t r[32];
+          fetch(c, r);
+          tmem_ld_wait();
+          hide_tail(c, r);
+          weigh(c, r, base2);
+        }
+      }
+#pragma unroll
+      for (int c = 0; c < 4; ++c) tmem_st_32x16(s_addr + c * 16, packed[c]);
       sum += sum2(add2(sums[0], sums[1]));
       if (visible < kXN && (kTwoRanges || t == 0)) {
         // value rows behind the last key are zero for the product, whatever the stage held before. (Both tiles' products of this
@@ -369,38 +380,72 @@ shared_prefix_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
       tmem_st_wait();
       tc_fence_before_sync();
       __syncwarp();
-      if (lane == 0) {
-        mbar_arrive(p_full + t);
-        if (j == 0) mbar_arrive(p_full + t);   // for the warp that rescales: nothing to do yet
-      }
+      if (lane == 0) mbar_arrive(p_full + t);
     }
     // ---- the row's range ----
-    const int token = token0_of(t) + row / G;
-    const bool mine = row < tile_rows && token < all_tokens;
-    const size_t range = (static_cast<size_t>(token) * p.Hq + kvh * G + row % G) * p.S + (kTwoRanges ? 2 * split + t : split);
-    if (ok && mine && (steps == 0 || p.kv_lens[token / p.T] - p.T + 1 < p.shared)) {
-      p.lse_part[range] = -INFINITY;   // (nothing in the odd steps; or the sequence ends inside the shared keys)
-    }
     if (ok && steps > 0) {
       ok = __all_sync(0xffffffffu, mbar_wait(o_full + t, 0, abort_flag, timeout_ns));
-      if (ok) {
-        tc_fence_after_sync();
-        const bool valid = mine && p.kv_lens[token / p.T] - p.T + 1 >= p.shared;
-        const float inv = 1.f / sum;   // at least one, or NaN
+      tc_fence_after_sync();
+    }
+    const int token = token0_of(t) + row / G;
+    const bool mine = row < tile_rows && token < all_tokens && (!kTwoRanges || t == 0);
+    const size_t range = (static_cast<size_t>(token) * p.Hq + kvh * G + row % G) * p.S + split;
+    float weight = 1.f, weight_odd = 0.f;   // of this tile's output and of the odd steps'
+    // (all products are done: the K ring holds the odd steps' output, row by row, its 16-byte chunks exchanged so that rows lie in all banks)
+    float4* odd = reinterpret_cast<float4*>(sK) + row * (D / 4);
+    if constexpr (kTwoRanges) {
+      const bool has_odd = n_steps > 1;
+      if (t == 1 && has_odd && ok) {
+        s_odd[row] = make_float2(ref, sum);
 #pragma unroll
-        for (int c = 0; c < D / 32; ++c) {
-          uint32_t o[32];
-          tmem_ld_32x32(o_addr + c * 32, o);
+        for (int c = 0; c < D / 16; ++c) {
+          uint32_t o[16];
+          tmem_ld_32x16(o_addr + c * 16, o);
           tmem_ld_wait();
 #pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            float v[8];
-#pragma unroll
-            for (int e = 0; e < 8; ++e) v[e] = __uint_as_float(o[q * 8 + e]) * inv;
-            if (valid) store_32_bytes(p.o_part + range * D + c * 32 + q * 8, v);
-          }
+          for (int q = 0; q < 4; ++q)
+            odd[(c * 4 + q) ^ (row & (D / 4 - 1))] = make_float4(__uint_as_float(o[4 * q]), __uint_as_float(o[4 * q + 1]), __uint_as_float(o[4 * q + 2]),
+                                                                 __uint_as_float(o[4 * q + 3]));
         }
-        if (valid) p.lse_part[range] = (ref + log2f(sum)) * 0.6931471805599453f;
+      }
+      asm volatile("bar.sync 1, 256;" ::: "memory");   // (both tiles' warps get here, after an abort too)
+      if (has_odd && *abort_flag == 0u) {
+        const float2 x = s_odd[row];
+        const float top = fmaxf(ref, x.x), base = top == -INFINITY ? 0.f : top;
+        weight = prefix_exp2(ref - base);
+        weight_odd = prefix_exp2(x.x - base);
+        sum = sum * weight + x.y * weight_odd;
+        ref = top;
+      }
+    }
+    if (ok && mine) {
+      if (steps == 0 || p.kv_lens[token / p.T] - p.T + 1 < p.shared) p.lse_part[range] = -INFINITY;   // (the sequence ends inside the shared keys)
+      else p.lse_part[range] = (ref + log2f(sum)) * 0.6931471805599453f;
+    }
+    if (ok && steps > 0 && !(kTwoRanges && t == 1)) {
+      const bool valid = mine && p.kv_lens[token / p.T] - p.T + 1 >= p.shared;
+      const float inv = 1.f / sum;
+#pragma unroll
+      for (int c = 0; c < D / 32; ++c) {
+        uint32_t o[32];
+        tmem_ld_32x32(o_addr + c * 32, o);
+        tmem_ld_wait();
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          float v[8];
+#pragma unroll
+          for (int e = 0; e < 8; ++e) v[e] = __uint_as_float(o[q * 8 + e]) * weight;
+          if (kTwoRanges && n_steps > 1) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              const float4 x = odd[(c * 8 + q * 2 + h) ^ (row & (D / 4 - 1))];
+              v[4 * h] += x.x * weight_odd; v[4 * h + 1] += x.y * weight_odd; v[4 * h + 2] += x.z * weight_odd; v[4 * h + 3] += x.w * weight_odd;
+            }
+          }
+#pragma unroll
+          for (int e = 0; e < 8; ++e) v[e] *= inv;
+          if (valid) store_32_bytes(p.o_part + range * D + c * 32 + q * 8, v);
+        }
       }
     }
   }
@@ -408,7 +453,7 @@ shared_prefix_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
   // ---------------------------------------------------------------------- teardown
   tc_fence_before_sync();
   __syncthreads();
-  if (warp == 15) tmem_dealloc(tmem_base, 512);
+  if (warp == 10) tmem_dealloc(tmem_base, 512);
   if (threadIdx.x == 0 && *abort_flag != 0u && p.status != nullptr) atomicMax(p.status, static_cast<uint32_t>(kStatusPipeTimeout));
 }
 
@@ -434,7 +479,7 @@ bool shared_prefix_tc_takes(const SharedPrefixParams& p, int D) {
          static_cast<long long>(p.num_blocks) * p.page < 0x7fffff00LL && p.Hkv <= 65535;
 }
 
-// p.prefix_splits ranges per row (twice as many as CTAs where all rows fit one tile), p.prefix_chunk keys (a multiple of 128) per CTA.
+// p.prefix_splits ranges of p.prefix_chunk keys (a multiple of 128).
 int shared_prefix_tc_launch(const SharedPrefixParams& p, int D, int dtype, cudaStream_t s) {
   const int G = p.Hq / p.Hkv, tile_tokens = kXM / G, tiles = (p.B * p.T + tile_tokens - 1) / tile_tokens;
   const bool two_ranges = tiles == 1;
@@ -445,7 +490,7 @@ int shared_prefix_tc_launch(const SharedPrefixParams& p, int D, int dtype, cudaS
   if (rc == kOk) rc = make_tma_3d(&tk, p.k_cache, dtype, D, p.Hkv, slots, D, static_cast<uint64_t>(p.Hkv) * D, 64, 1, rows, true);
   if (rc == kOk) rc = make_tma_3d(&tv, p.v_cache, dtype, D, p.Hkv, slots, D, static_cast<uint64_t>(p.Hkv) * D, 64, 1, rows, true);
   if (rc != kOk) return rc;
-  const dim3 grid(two_ranges ? p.prefix_splits / 2 : p.prefix_splits, two_ranges ? 1 : (tiles + 1) / 2, p.Hkv);
+  const dim3 grid(p.prefix_splits, two_ranges ? 1 : (tiles + 1) / 2, p.Hkv);
   B200_REQUIRE(grid.y <= 65535, "shared-prefix attention: too many rows");
 #define B200_PREFIX(A, TWO) (dtype == kBF16 ? launch_prefix<A, true, TWO>(tq, tk, tv, p, grid, s) : launch_prefix<A, false, TWO>(tq, tk, tv, p, grid, s))
   if (D == 128) return two_ranges ? B200_PREFIX(2, true) : B200_PREFIX(2, false);

@@ -1038,9 +1038,9 @@ def choose_prefix_splits(batch: int, tokens: int, heads: int, kv_heads: int, sha
         own_splits += 1
     tiles = -(-batch * tokens // (128 // group))
     units, steps = kv_heads * -(-tiles // 2), -(-shared // 128)
-    step_us, merge_us = (1.1 if tiles == 1 else 2.2) * dim / 128, (2 if tiles == 1 else 1) * batch * tokens * heads * dim * 8 / 3e6
+    step_us, merge_us = (0.8 if tiles == 1 else 1.6) * dim / 128, batch * tokens * heads * dim * 8 / 3e6
     best = min((-(-units * r // sm_count) * (-(-steps // r) * step_us + 6) + r * merge_us, r) for r in range(1, min(steps, 64) + 1))[1]
-    return True, best * (2 if tiles == 1 else 1), own_splits
+    return True, best, own_splits
 
 
 def shared_prefix_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, kv_lens: torch.Tensor, block_table: torch.Tensor,
