@@ -62,6 +62,8 @@ def test_shared_prefix_attention_refuses():
     _refused(TypeError, call, block_table=ok["block_table"].long())
     _refused(ValueError, call, tokens=3)
     _refused(ValueError, call, tokens=0)
+    _refused(ValueError, call, scale=0.0)
+    _refused(ValueError, call, scale=float("nan"))
     _refused(ValueError, call, shared=-1)
     _refused(ValueError, call, shared=49)                                  # the table has three pages
     _refused(ValueError, call, q=ok["q"][:, :3])                           # three query heads for two of the cache

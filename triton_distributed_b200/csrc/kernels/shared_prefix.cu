@@ -446,6 +446,7 @@ B200_API int b200_shared_prefix_attention(const void* q, long long ldq, const vo
   B200_REQUIRE(D == 64 || D == 128, "shared-prefix attention supports head sizes 64 and 128, got %d", D);
   B200_REQUIRE(Hkv > 0 && Hq > 0 && Hq % Hkv == 0, "Hq (%d) must be a multiple of Hkv (%d)", Hq, Hkv);
   B200_REQUIRE(B >= 0 && T >= 1 && page >= 1 && num_blocks >= 1 && width >= 0 && shared >= 0 && ldq % 8 == 0, "shared-prefix attention: bad sizes");
+  B200_REQUIRE(scale > 0.f, "the score scale must be positive");
   B200_REQUIRE(own_splits >= 1 && (shared == 0 ? prefix_splits == 0 : prefix_splits >= 1), "shared-prefix attention: bad split counts");
   if (B == 0) return kOk;
   cudaStream_t s = static_cast<cudaStream_t>(stream);

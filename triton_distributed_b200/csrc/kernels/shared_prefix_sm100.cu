@@ -14,7 +14,7 @@
 // Tensor memory: S of tile t at columns 128 t, O of tile t at 256 + 128 t. P is written over S as 16-bit pairs and is the A operand of
 // the second product; V is read in place as an MN-major B operand.
 // The softmax of a step does not wait for its maximum: the weights are taken against the reference of the steps before, and only if one of
-// a warp's comes out above 2^8 (or at the first step) the warp raises its rows' references to their maxima, rescales their output and takes the step's
+// a warp's scores lies above it by more than 8 (or at the first step) the warp raises its rows' references to their maxima, rescales their output and takes the step's
 // weights anew from the scores, which are still there because the weights stay in registers until then. Over a long range the maximum of the first
 // steps stands, so this is rare, and the chain of a step is one pass over the scores instead of two. Weights above one are rounded like those
 // below (relative to themselves); what is lost is that a row's largest weight was held exactly: error against 64 bits 2.3e-3 of the norm before and now.
@@ -33,18 +33,23 @@ constexpr int kXM = 128, kXN = 128;            // rows per tile, keys per step
 constexpr int kXAtom = 128 * 64 * 2;           // 128 rows x 64 columns of 16 bits: 16 KB
 constexpr int kXThreads = 384;
 constexpr int kXSoftmaxRegs = 208, kXOtherRegs = 88;   // 256 x 208 + 128 x 88 = 384 x 168, what the block starts with
-constexpr float kXRaise = 256.f;               // a weight above it raises the reference (f16 holds 2^8 times as much)
+constexpr float kXRaise = 8.f;                 // a score so far above the reference raises it (weights up to 2^8; f16 holds 2^8 times as much)
 template <int kAtoms, bool kTwoRanges>
 struct PrefixShape {
   static constexpr int kTile = kAtoms * kXAtom;
   static constexpr int kQTiles = kTwoRanges ? 1 : 2;
   static constexpr int kStages = kTwoRanges ? (kAtoms == 2 ? 3 : 4) : (kAtoms == 2 ? 2 : 4);   // of K, and as many of V
-  static constexpr int kSmem = kQTiles * kTile + 2 * kStages * kTile + 1024 /*alignment*/ + 256 /*barriers*/ + kXM * 8 /*maxima and sums of the odd steps*/;
+  static constexpr int kSmem = kQTiles * kTile + 2 * kStages * kTile + 1024 /*alignment*/ + 256 /*barriers*/ + kXM * 8 /*references and sums of the odd steps*/;
 };
 
 __device__ __forceinline__ float prefix_exp2(float x) {   // one instruction; -inf gives 0
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float max3_nan(float a, float b, float c) {   // NaN if one of them is
+  float y;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
   return y;
 }
 __device__ __forceinline__ void store_32_bytes(float* dst, const float (&v)[8]) {
@@ -277,9 +282,8 @@ shared_prefix_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
       const int visible = key1 - key0 - c_step * kXN;
       uint32_t packed[4][16];
       f32x2 sums[2];
-      // scores 32 c ... of the row, those behind the last key at -inf
       auto fetch = [&](int c, uint32_t (&r)[32]) { tmem_ld_32x32(s_addr + c * 32, r); };
-      auto hide_tail = [&](int c, uint32_t (&r)[32]) {
+      auto hide_tail = [&](int c, uint32_t (&r)[32]) {   // scores behind the last key
         if (visible < (c + 1) * 32) {
 #pragma unroll
           for (int e = 0; e < 32; ++e)
@@ -297,6 +301,7 @@ shared_prefix_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
           packed[c][e] = BF16 ? pack_bf16x2(p0, p1) : pack_f16x2(p0, p1);
         }
       };
+      float mx = -INFINITY;   // of the scores; NaN if one of them is
       bool raise = j == 0;
       if (j > 0) {
         sums[0] = sums[1] = pack2(0.f, 0.f);
@@ -309,23 +314,11 @@ shared_prefix_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
           if (c < 3) fetch(c + 1, r[(c + 1) & 1]);
           hide_tail(c, r[c & 1]);
           weigh(c, r[c & 1], base2);
-        }
-        float most = 0.f;
-        if (BF16) {
-          __nv_bfloat162 m = *reinterpret_cast<__nv_bfloat162*>(&packed[0][0]);
 #pragma unroll
-          for (int e = 1; e < 64; ++e) m = __hmax2(m, *reinterpret_cast<__nv_bfloat162*>(&packed[e >> 4][e & 15]));
-          most = fmaxf(__low2float(m), __high2float(m));
-        } else {
-          __half2 m = *reinterpret_cast<__half2*>(&packed[0][0]);
-#pragma unroll
-          for (int e = 1; e < 64; ++e) m = __hmax2(m, *reinterpret_cast<__half2*>(&packed[e >> 4][e & 15]));
-          most = fmaxf(__low2float(m), __high2float(m));
+          for (int e = 0; e < 32; e += 2) mx = max3_nan(mx, __uint_as_float(r[c & 1][e]), __uint_as_float(r[c & 1][e + 1]));
         }
-        raise = __any_sync(0xffffffffu, most > kXRaise || ref == -INFINITY);
-      }
-      if (raise) {
-        float mx = -INFINITY;
+        raise = __any_sync(0xffffffffu, !(mx * p.scale_log2e - ref <= kXRaise));   // (also without a reference, and with NaN)
+      } else {
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
           uint32_t r[32];
@@ -333,8 +326,10 @@ shared_prefix_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
           tmem_ld_wait();
           hide_tail(c, r);
 #pragma unroll
-          for (int e = 0; e < 32; ++e) mx = fmaxf(mx, __uint_as_float(r[e]));
+          for (int e = 0; e < 32; e += 2) mx = max3_nan(mx, __uint_as_float(r[e]), __uint_as_float(r[e + 1]));
         }
+      }
+      if (raise) {
         const float top = fmaxf(ref, mx * p.scale_log2e), base = top == -INFINITY ? 0.f : top;
         const float corr = ref == -INFINITY ? 0.f : prefix_exp2(ref - base);
         ref = top;
@@ -426,25 +421,26 @@ shared_prefix_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
       const bool valid = mine && p.kv_lens[token / p.T] - p.T + 1 >= p.shared;
       const float inv = 1.f / sum;
 #pragma unroll
-      for (int c = 0; c < D / 32; ++c) {
-        uint32_t o[32];
-        tmem_ld_32x32(o_addr + c * 32, o);
+      for (int c = 0; c < D / 16; ++c) {
+        const int col = c * 16;
+        uint32_t o[16];
+        tmem_ld_32x16(o_addr + col, o);
         tmem_ld_wait();
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
+        for (int q = 0; q < 2; ++q) {
           float v[8];
 #pragma unroll
           for (int e = 0; e < 8; ++e) v[e] = __uint_as_float(o[q * 8 + e]) * weight;
           if (kTwoRanges && n_steps > 1) {
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-              const float4 x = odd[(c * 8 + q * 2 + h) ^ (row & (D / 4 - 1))];
+              const float4 x = odd[(col / 4 + q * 2 + h) ^ (row & (D / 4 - 1))];
               v[4 * h] += x.x * weight_odd; v[4 * h + 1] += x.y * weight_odd; v[4 * h + 2] += x.z * weight_odd; v[4 * h + 3] += x.w * weight_odd;
             }
           }
 #pragma unroll
           for (int e = 0; e < 8; ++e) v[e] *= inv;
-          if (valid) store_32_bytes(p.o_part + range * D + c * 32 + q * 8, v);
+          if (valid) store_32_bytes(p.o_part + range * D + col + q * 8, v);
         }
       }
     }
@@ -465,6 +461,10 @@ static int launch_prefix(const CUtensorMap& tq, const CUtensorMap& tk, const CUt
   B200_CHECK_CUDA(cudaGetDevice(&dev));
   auto kernel = shared_prefix_kernel<kAtoms, BF16, kTwoRanges>;
   if (!configured[dev & 63]) {
+    cudaFuncAttributes attr;
+    B200_CHECK_CUDA(cudaFuncGetAttributes(&attr, kernel));   // the warps' register shares must not exceed what the block starts with
+    if (attr.numRegs * kXThreads < 256 * kXSoftmaxRegs + 128 * kXOtherRegs)
+      return set_error(kErrUnsupported, "shared-prefix kernel was compiled for %d registers", attr.numRegs);
     B200_CHECK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem));
     configured[dev & 63] = true;
   }

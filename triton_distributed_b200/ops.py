@@ -1083,6 +1083,8 @@ def shared_prefix_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: tor
     if per_element != 1 or (Hq > 1 and per_head != D) or ldq % 8 or ldq < 0 or (at_q | at_k | at_v) % 16:
         raise ValueError("shared_prefix_attention: q holds whole rows of heads, a multiple of 8 elements apart; q and caches start on 16 bytes")
     blocks = -(-shared // page)
+    if not scale > 0:
+        raise ValueError("shared_prefix_attention: the score scale must be positive")
     if shared < 0 or (shared > 0 and prefix_table is None and (width < blocks or B == 0)):
         raise ValueError(f"shared_prefix_attention: {shared} shared keys do not fit the block table")
     if prefix_table is not None and (prefix_table.dim() != 1 or prefix_table.shape[0] < blocks or not prefix_table.is_contiguous()):
