@@ -33,8 +33,12 @@ constexpr int kSpanThreads = 128;
 constexpr int kSpanSlice = 16;   // keys per slice of a warp
 constexpr int kSpanRing = 3;     // slices in flight per warp
 
+constexpr int kSpanMostRows = 32;   // per CTA
 template <int D>
-constexpr int span_smem() { return 4 * kSpanRing * 2 * kSpanSlice * D * 2; }
+constexpr int span_smem() {         // the rings; in the end the four warps' maxima, sums and outputs (rows D + 4 floats apart)
+  constexpr int rings = 4 * kSpanRing * 2 * kSpanSlice * D * 2, merge = 4 * kSpanMostRows * (2 + D + 4) * 4;
+  return rings > merge ? rings : merge;
+}
 
 __device__ __forceinline__ float span_exp2(float x) {   // one instruction; -inf gives 0
   float y;
@@ -276,6 +280,7 @@ __device__ __forceinline__ void span_body(const SharedPrefixParams& p, uint8_t* 
   __syncthreads();  // all rings are idle: their memory becomes the merge area
 
   // ---- merge of the four warps ----
+  static_assert(NB * 8 <= kSpanMostRows, "the merge area holds the rows of a CTA");
   constexpr int kRows = NB * 8, kPitch = D + 4;      // (lanes of one store are columns of four rows: 4 words apart in the banks)
   float* red_m = reinterpret_cast<float*>(smem);     // [4][rows]
   float* red_l = red_m + 4 * kRows;                  // [4][rows]
@@ -359,7 +364,9 @@ __global__ void __launch_bounds__(kSpanThreads) shared_prefix_span_kernel(const 
   const int t0 = start + split * chunk, t1 = min(len, t0 + chunk);
   span_body<BF16, D, NBO>(p, smem, kvh, b * p.T, group * NBO * 8, rows, p.block_table + static_cast<size_t>(b) * p.bt_stride, p.width, t0, t1,
                           true, len - p.T + 1, p.prefix_splits + split);
-  if (p.late_wait) griddep_wait();   // the kernel in front (the shared keys') is complete before this one is
+  // The kernel in front (the shared keys') has to be complete before this one is. One CTA sees to that: if all of them waited, they would keep the
+  // SMs that the kernel in front leaves free (64 / 8 heads, batch 64, with 64 CTAs in front: 155 us for 130).
+  if (p.late_wait && blockIdx.x == gridDim.x - 1) griddep_wait();
 }
 
 // The merge: a warp per row, the weights of up to 32 ranges at a time in its lanes.
