@@ -109,15 +109,17 @@ __device__ __forceinline__ void span_body(const SharedPrefixParams& p, uint8_t* 
       const uint32_t slot = ring + (j % kSpanRing) * (2 * kSliceBytes);
       const int blk = next_blk;
       if (page_fast && j + 1 < mine) next_blk = page_of(st0 + 4 * kSpanSlice);
-      if (page_fast && blk >= 0 && st0 >= t0 && st0 + kSpanSlice <= t1) {
-        const size_t off = (static_cast<size_t>(blk) * p.page + st0 % p.page) * token_bytes + lane_off;
+      if (page_fast) {
+        const bool all = blk >= 0 && st0 >= t0 && st0 + kSpanSlice <= t1;
+        const size_t off = (static_cast<size_t>(max(blk, 0)) * p.page + st0 % p.page) * token_bytes + lane_off;
         const uint8_t *ks = kc + off, *vs = vc + off;
 #pragma unroll
         for (int i = 0; i < kCopies; ++i) {
-          const int tok_in = i * kLaneRows + hi;
+          const int tok_in = i * kLaneRows + hi, tok = st0 + tok_in;
           const uint32_t at = slot + tok_in * kRowBytes + ((chunk ^ (tok_in & 7)) * 16);
-          cp_async_16(at, ks + i * step, 16);
-          cp_async_16(at + kSliceBytes, vs + i * step, 16);
+          const int bytes = all || (blk >= 0 && tok >= t0 && tok < t1) ? 16 : 0;   // (the address is inside the page either way)
+          cp_async_16(at, ks + i * step, bytes);
+          cp_async_16(at + kSliceBytes, vs + i * step, bytes);
         }
       } else {
 #pragma unroll 1
@@ -302,6 +304,7 @@ __device__ __forceinline__ void span_body(const SharedPrefixParams& p, uint8_t* 
     }
   __syncthreads();
   constexpr int kVecs = D / 4;
+#pragma unroll 4
   for (int i = threadIdx.x; i < nrows * kVecs; i += kSpanThreads) {
     const int r = i / kVecs, c = i - r * kVecs;
     float top = -INFINITY;

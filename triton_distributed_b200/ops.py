@@ -1017,9 +1017,12 @@ def choose_prefix_splits(batch: int, tokens: int, heads: int, kv_heads: int, sha
                          dim: int = 128, sm_count: int = 148, variant: str | None = None) -> tuple[bool, int, int]:
     """(tensor-core kernel for the shared keys, ranges of the shared keys, ranges of everybody's own keys) for `shared_prefix_attention`.
 
-    Warp kernel: one wave of two CTAs per SM, all with about as many keys, at least 128. Tensor-core kernel: the number of ranges with the least
-    estimated time, from what a step of 128 keys, a CTA's start and end (6 us) and the partial results of one more range (written and read at 3 TB/s)
-    take; own keys are split only while that leaves SMs without work."""
+    The tensor-core kernel from 17 rows per KV head on (us, warp and tensor-core kernel, 64 / 8 heads of 128, 2048 and 65536 keys: 16 rows 12.1 and 14.0,
+    55.6 and 58.2; 24 rows 15.6 and 14.0, 78.4 and 57.8; 64 rows 17.7 and 14.0, 220 and 59; 14 / 2 heads of 64, 21 rows: 10.2 and 11.2, 35.3 and 24.3).
+    Warp kernel: one wave of two CTAs per SM, ranges of at least 128 keys. Tensor-core kernel: the number of ranges with the least
+    estimated time, from what was measured: a step of 128 keys, a CTA's start and end (6 us), the partial results of one more range (written and read
+    at 3 TB/s), and the own keys' CTAs (5 us and 18 ns a key), which run on the SMs that the shared keys leave and behind them. Own keys are split only
+    while that leaves SMs without work."""
     group = heads // kv_heads
     rows = batch * tokens * group
     blocks = lambda n: -(-n // (8 if n <= 8 else 16 if n <= 16 else 32))  # noqa: E731  (CTAs for n rows of the warp kernel)
@@ -1027,20 +1030,28 @@ def choose_prefix_splits(batch: int, tokens: int, heads: int, kv_heads: int, sha
     able = shared > 0 and group <= 128 and page >= 8 and (page % 128 == 0 or 128 % page == 0) and slots < 0x7fffff00 and kv_heads <= 65535
     if variant == "tc" and not able:
         raise ValueError("shared_prefix_attention: these heads or pages are not for the tensor-core kernel")
-    tc = able and (rows > 32 if variant is None else variant == "tc")
+    tc = able and (rows > 16 if variant is None else variant == "tc")
     if not tc:
-        prefix_ctas = kv_heads * blocks(rows) if shared else 0
-        share = max(128, (prefix_ctas * shared + own_ctas * own) // (2 * sm_count))
-        chunk = -(-share // 64) * 64
-        return False, min(64, -(-shared // chunk)) if shared else 0, max(1, min(64, -(-own // chunk)))
+        prefix_ctas, slots = kv_heads * blocks(rows) if shared else 0, 2 * sm_count
+        prefix_splits = 0
+        if shared:
+            free = slots - own_ctas if own_ctas <= sm_count else slots * prefix_ctas * shared // (prefix_ctas * shared + own_ctas * own)
+            prefix_splits = max(1, min(64, -(-shared // 128), free // prefix_ctas))
+        return False, prefix_splits, max(1, min(64, -(-own // 128), (slots - prefix_ctas * prefix_splits) // own_ctas))
     own_splits = 1
     while own_splits < 64 and own_ctas * own_splits < sm_count // 2 and own > 256 * own_splits:
         own_splits += 1
     tiles = -(-batch * tokens // (128 // group))
-    units, steps = kv_heads * -(-tiles // 2), -(-shared // 128)
-    step_us, merge_us = (0.8 if tiles == 1 else 1.6) * dim / 128, batch * tokens * heads * dim * 8 / 3e6
-    best = min((-(-units * r // sm_count) * (-(-steps // r) * step_us + 6) + r * merge_us, r) for r in range(1, min(steps, 64) + 1))[1]
-    return True, best, own_splits
+    units, steps, ctas = kv_heads * -(-tiles // 2), -(-shared // 128), own_ctas * own_splits
+    step_us, merge_us = 0.95 if tiles == 1 else 1.9, batch * tokens * heads * dim * 8 / 3e6
+    own_us = 5 + 0.018 * own / 2 / own_splits
+
+    def estimate(r: int) -> float:
+        us = -(-units * r // sm_count) * (-(-steps // r) * step_us + 6)
+        rest = ctas - int(2 * max(0, sm_count - units * r) * us / own_us)   # own CTAs that find no SM beside the shared keys' in time
+        return max(us, own_us) + (max(1.0, rest / (2 * sm_count)) * own_us if rest > 0 else 0.0) + r * merge_us
+
+    return True, min(range(1, min(steps, 64) + 1), key=estimate), own_splits
 
 
 def shared_prefix_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, kv_lens: torch.Tensor, block_table: torch.Tensor,
