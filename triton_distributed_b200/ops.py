@@ -981,6 +981,13 @@ def _check_device(name: str, *tensors: torch.Tensor | None) -> int:
     return current
 
 
+def _status_word(device: torch.device) -> torch.Tensor | None:
+    """``_pipeline_status``, but None where it would have to be made inside a capture (call an op of this kind once before)."""
+    if device.index not in _pipe_status and torch.cuda.is_current_stream_capturing():
+        return None
+    return _pipeline_status(device)
+
+
 _P, _I, _L = ctypes.c_void_p, ctypes.c_int, ctypes.c_longlong
 # what the entry points of this section take: with these known, plain numbers are passed without an object for each
 _SERVING_ARGS = {
@@ -1062,8 +1069,8 @@ def shared_prefix_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: tor
 
     q [B * tokens, Hq, D], 16-bit, rows may be strided; caches [num_blocks, page, Hkv, D] in the type of q, D 64 or 128; kv_lens int32 [B] with the
     new tokens; block_table int32 [B, max_blocks]. Query token t of sequence b attends keys j < kv_lens[b] - tokens + t + 1; a row
-    without any gives zeros. Keys j < ``shared`` are read through ``prefix_table`` (int32 [>= ceil(shared / page)], default: the first
-    sequence's row of the block table) for every sequence that reaches beyond them with all its tokens; shorter sequences (also
+    without any gives zeros. What is not a page of the cache, or lies behind the table, counts as keys and values of zero. Keys j < ``shared`` are read through ``prefix_table`` (int32 [>= ceil(shared / page)], default: the first
+    row of the block table, which has to hold them then) for every sequence that reaches beyond them with all its tokens; shorter sequences (also
     kv_lens 0) are attended over their own table alone. ``shared`` need not be a multiple of the page. ``max_kv_len``: an upper bound on kv_lens for the choice
     of splits (default: what the table can hold). ``variant``: which kernel reads the shared keys, "warp" (warp-level products, any page) or "tc" (tcgen05 tiles; pages
     that 128 is a multiple of, or that are multiples of 128); None picks by the rows per KV head. Returns [B * tokens, Hq, D] (and the natural-log LSE fp32 [B * tokens, Hq])."""
@@ -1104,7 +1111,7 @@ def shared_prefix_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: tor
         raise ValueError("shared_prefix_attention: the output is contiguous and has the shape and type of q")
     device = _check_device("shared_prefix_attention", q, k_cache, v_cache, kv_lens, block_table, prefix_table, out)
     if out is None:
-        out = q.new_empty((T, Hq, D))
+        out = torch.empty_like(q) if ldq == Hq * D else q.new_empty((T, Hq, D))
     lse = q.new_empty((T, Hq), dtype=torch.float32) if return_lse else None
     if B:
         longest = width * page if max_kv_len is None else min(int(max_kv_len), width * page)
@@ -1115,7 +1122,7 @@ def shared_prefix_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: tor
         table = block_table.data_ptr()
         _launch("b200_shared_prefix_attention", 3 if tc else 2, device, at_q, ldq, at_k, at_v, kv_lens.data_ptr(), table, ldt, width,
                 table if prefix_table is None else prefix_table.data_ptr(), B, tokens, Hq, Hkv, D, N, page, shared, scale, tc, prefix_splits, own_splits, at,
-                at + ranges * D * 4, out.data_ptr(), _dptr(lse), dtype_code(dtype), _pipeline_status(q.device).data_ptr())
+                at + ranges * D * 4, out.data_ptr(), _dptr(lse), dtype_code(dtype), _dptr(_status_word(q.device)))
     return (out, lse) if return_lse else out
 
 
@@ -1205,6 +1212,7 @@ def fork_pages(block_table: torch.Tensor, kv_lens: torch.Tensor, refs: torch.Ten
     and hold the pages of the source's tokens (``refs`` counts how many entries hold a page). All sources are read as they were before the
     call, so rows can be exchanged; pairs with a row outside the table and all but the first pair of a destination are skipped. The page that the source's last token is in is shared too:
     ``reserve_pages`` copies it for whoever writes next. src, dst: whole numbers [n], lists or tensors."""
+    page_size = int(page_size)
     R, W, N = _check_page_state("fork_pages", block_table, refs, kv_lens, page_size)
     src, dst = _rows("fork_pages", src, block_table.device), _rows("fork_pages", dst, block_table.device)
     if src.shape != dst.shape:
@@ -1212,14 +1220,15 @@ def fork_pages(block_table: torch.Tensor, kv_lens: torch.Tensor, refs: torch.Ten
     device = _check_device("fork_pages", block_table, kv_lens, refs, src, dst)
     n = src.shape[0]
     if n:
-        scratch = refs.new_empty(n * (W + 1))
-        _launch("b200_fork_pages", 2, device, block_table.data_ptr(), kv_lens.data_ptr(), refs.data_ptr(), src.data_ptr(), dst.data_ptr(), n, R, W, N, page_size,
-                scratch.data_ptr())
+        scratch = None if n <= 256 and n * W <= 8192 else refs.new_empty(n * (W + 1))   # as few are one launch
+        _launch("b200_fork_pages", 1 if scratch is None else 2, device, block_table.data_ptr(), kv_lens.data_ptr(), refs.data_ptr(), src.data_ptr(), dst.data_ptr(), n,
+                R, W, N, page_size, _dptr(scratch))
 
 
 def trim_pages(block_table: torch.Tensor, kv_lens: torch.Tensor, refs: torch.Tensor, page_size: int, lens: torch.Tensor | None = None, rows=None) -> None:
     """Rows keep their first ``lens`` tokens (int32 [n]; None: none) and the pages of these, in place: drafts that were refused, sequences that are
     over. ``rows`` [n] (default: all): which; a length below zero leaves a row alone, one above a row's length takes back unused room only."""
+    page_size = int(page_size)
     R, W, N = _check_page_state("trim_pages", block_table, refs, kv_lens, page_size)
     rows = _rows("trim_pages", rows, block_table.device) if rows is not None else None
     n = R if rows is None else rows.shape[0]
@@ -1248,8 +1257,10 @@ def reserve_pages(block_table: torch.Tensor, kv_lens: torch.Tensor, refs: torch.
         counts, count = count, 0
         if counts.dtype != torch.int32 or counts.shape != (R,) or not counts.is_contiguous():
             raise ValueError("reserve_pages: one count (int32) for every row")
-    elif count < 0 or count >= 1 << 30:
-        raise ValueError("reserve_pages: the count of tokens is not negative")
+    else:
+        count = int(count)
+        if count < 0 or count >= 1 << 30:
+            raise ValueError("reserve_pages: the count of tokens is not negative")
     if status is not None and (status.dtype != torch.int32 or status.numel() != 1):
         raise ValueError("reserve_pages: the status is one int32")
     device = _check_device("reserve_pages", block_table, kv_lens, refs, counts, status, *caches)
