@@ -128,7 +128,7 @@ shared_prefix_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
   if (warp >= 8) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kXOtherRegs));
     if (warp == 8) {
-      // ---------------------------------------------------------------- TMA producer: the warp reads page numbers, lane 0 copies
+      // ---------------------------------------------------------------- TMA producer: the warp reads page numbers, every lane copies a part of a step
       const int rows = min(p.page, kXN), pieces = kXN / rows;   // keys per copy, copies per step
       const int piece0 = key0 / rows, piece_end = (p.shared + rows - 1) / rows;   // copies are numbered from the first key on
       auto page_at = [&](int piece) -> int {   // first slot of a copy (behind the cache's end where there is no such page)
@@ -147,6 +147,7 @@ shared_prefix_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
 #pragma unroll
             for (int a = 0; a < kAtoms; ++a) tma_load_3d(sQ + t * kTile + a * kXAtom, &tmQ, q_full, 64 * a, kvh * G, token0_of(t));
       }
+      const int piece = lane / kAtoms, atom = lane % kAtoms;   // each lane makes one copy of a step (24 x 5 drafts, pages of 16: 33.5 us, 40 with one lane for all)
       int done = 0;
       for (int j = 0; j < n_steps; ++j) {
         const int st = j % kSt;
@@ -156,24 +157,17 @@ shared_prefix_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
           now = next;
           next = page_at(window + 32 + lane);
         }
+        const int slot = __shfl_sync(0xffffffffu, now, first - window + piece);   // (of the lanes' copies; behind the step's last one unused)
         ok = mbar_wait(k_empty + st, ((j / kSt) & 1) ^ 1, abort_flag, timeout_ns);
         if (!__all_sync(0xffffffffu, ok)) break;
         if (lane == 0) mbar_expect_tx(k_full + st, n * rows * 128 * kAtoms);
-        for (int i = 0; i < n; ++i) {
-          const int slot = __shfl_sync(0xffffffffu, now, first - window + i);
-          if (lane == 0)
-#pragma unroll
-            for (int a = 0; a < kAtoms; ++a) tma_load_3d(sK + st * kTile + a * kXAtom + i * rows * 128, &tmK, k_full + st, 64 * a, kvh, slot);
-        }
+        __syncwarp();
+        if (piece < n) tma_load_3d(sK + st * kTile + atom * kXAtom + piece * rows * 128, &tmK, k_full + st, 64 * atom, kvh, slot);
         ok = mbar_wait(v_empty + st, ((j / kSt) & 1) ^ 1, abort_flag, timeout_ns);
         if (!__all_sync(0xffffffffu, ok)) { done = -(j + 1); break; }   // (K of this step is on its way)
         if (lane == 0) mbar_expect_tx(v_full + st, n * rows * 128 * kAtoms);
-        for (int i = 0; i < n; ++i) {
-          const int slot = __shfl_sync(0xffffffffu, now, first - window + i);
-          if (lane == 0)
-#pragma unroll
-            for (int a = 0; a < kAtoms; ++a) tma_load_3d(sV + st * kTile + a * kXAtom + i * rows * 128, &tmV, v_full + st, 64 * a, kvh, slot);
-        }
+        __syncwarp();
+        if (piece < n) tma_load_3d(sV + st * kTile + atom * kXAtom + piece * rows * 128, &tmV, v_full + st, 64 * atom, kvh, slot);
         done = j + 1;
       }
       // after an abort nothing waits for the last copies any more: they have to land before shared memory is given back
