@@ -69,6 +69,7 @@ def test_shared_prefix_attention_refuses():
     _refused(ValueError, call, q=ok["q"][:, :3])                           # three query heads for two of the cache
     _refused(ValueError, call, q=ok["q"][..., :32])
     _refused(ValueError, call, q=ok["q"].transpose(0, 1))
+    _refused(ValueError, call, q=ok["q"][:1].expand(4, 4, 64))
     _refused(ValueError, call, kv_lens=ok["kv_lens"][:1])
     _refused(ValueError, call, k_cache=ok["k_cache"][:, ::2], v_cache=ok["v_cache"][:, ::2])
     _refused(ValueError, call, prefix_table=ok["block_table"][0, :1])      # two pages are shared

@@ -1098,7 +1098,7 @@ def shared_prefix_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: tor
         raise ValueError("shared_prefix_attention needs contiguous caches and lengths and a row-major block table")
     if T <= 1:
         ldq = Hq * D
-    if per_element != 1 or (Hq > 1 and per_head != D) or ldq % 8 or ldq < 0 or (at_q | at_k | at_v) % 16:
+    if per_element != 1 or (Hq > 1 and per_head != D) or ldq % 8 or ldq < Hq * D or (at_q | at_k | at_v) % 16:
         raise ValueError("shared_prefix_attention: q holds whole rows of heads, a multiple of 8 elements apart; q and caches start on 16 bytes")
     blocks = -(-shared // page)
     if not scale > 0:
@@ -1115,7 +1115,9 @@ def shared_prefix_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: tor
     lse = q.new_empty((T, Hq), dtype=torch.float32) if return_lse else None
     if B:
         longest = width * page if max_kv_len is None else min(int(max_kv_len), width * page)
-        tc, prefix_splits, own_splits = choose_prefix_splits(B, tokens, Hq, Hkv, shared, max(1, longest - shared), page, N * page, D, variant=variant)
+        # (of lengths in steps, so that a sequence that grows finds the choice of the step before)
+        tc, prefix_splits, own_splits = choose_prefix_splits(B, tokens, Hq, Hkv, -(-shared // 128) * 128, max(64, -(-(longest - shared) // 64) * 64), page, N * page, D,
+                                                             variant=variant)
         ranges = T * Hq * (prefix_splits + own_splits)
         part = q.new_empty(ranges * (D + 1), dtype=torch.float32)   # outputs of all ranges, then their log-sum-exps
         at = part.data_ptr()
