@@ -141,11 +141,11 @@ def test_pool_slots():
     assert pool.slots(3).tolist() == [3 * 16 + 15, 5 * 16, 5 * 16 + 1, spare, spare + 1, spare + 2, spare, spare + 1, spare + 2]
 
 
-@pytest.mark.parametrize("B,T,heads,kv,shared,own,page", [(1, 1, 8, 8, 0, 1, 64), (256, 1, 8, 1, 131072, 256, 128), (64, 1, 64, 8, 32768, 1024, 64), (3, 8, 28, 4, 100, 50, 48),
+@pytest.mark.parametrize("B,T,heads,kv,shared,own,page", [(1, 1, 8, 8, 0, 1, 64), (256, 1, 8, 1, 131072, 256, 128), (64, 1, 64, 8, 32768, 1024, 64), (3, 8, 28, 4, 100, 50, 44),
                                                           (4, 1, 64, 8, 9000, 10, 16), (1, 300, 4, 4, 5, 1, 8)])
 @pytest.mark.parametrize("variant", [None, "warp", "tc"])
 def test_prefix_splits_cover_the_keys(B, T, heads, kv, shared, own, page, variant):
-    if variant == "tc" and (shared == 0 or page == 48):
+    if variant == "tc" and (shared == 0 or page == 44):
         with pytest.raises(ValueError):
             ops.choose_prefix_splits(B, T, heads, kv, shared, own, page, variant=variant)
         return

@@ -24,7 +24,7 @@ from ..utils import perf_func_cold
 
 OPS = ["decode_step", "prefill_attn", "gemm_skinny_fused", "ag_gemm", "gemm_rs", "grouped_gemm", "grouped_gemm_fp8", "ag_group_gemm", "moe_reduce_rs", "allreduce_rmsnorm", "ep_dispatch_combine",
        "decode_attn", "sp_decode", "moe_sort", "sampling", "rmsnorm", "qk_norm_rope",
-       "latent_decode", "residual_norm", "wkv", "gated_delta"]
+       "latent_decode", "residual_norm", "wkv", "gated_delta", "shared_prefix", "verify_drafts", "page_fork"]
 
 
 def main() -> None:
@@ -194,6 +194,36 @@ def main() -> None:
             fn = lambda: ops.gated_delta(rows[0][:, : H // 2 * D], rows[1][:, : H // 2 * D], rows[2], ab[:, :H], ab[:, H:], rows[3], c[:H], c[:H], c[:D],
                                          st, D, D, 1e-6, settled=True)
         info = {"flops": (5.0 if args.op == "wkv" else 7.0) * B * S * H * D * D}
+    elif args.op == "shared_prefix":  # 32 samples of a prompt of --kv-len tokens, 512 tokens of their own each
+        B, Hq, Hkv, D, page, own = 32, 64, 8, 128, 64, 512
+        common, width = args.kv_len // page, args.kv_len // page + own // page
+        N = common + B * (width - common)
+        k, v = (torch.randn(N, page, Hkv, D, device=dev, dtype=dt) for _ in range(2))
+        bt = torch.empty(B, width, device=dev, dtype=torch.int32)
+        bt[:, :common] = torch.arange(common, device=dev)
+        bt[:, common:] = torch.arange(common, N, device=dev).view(B, -1)
+        q, lens = torch.randn(B, Hq, D, device=dev, dtype=dt), torch.full((B,), width * page, device=dev, dtype=torch.int32)
+        fn = lambda: ops.shared_prefix_attention(q, k, v, lens, bt, common * page, 1 / math.sqrt(D))
+        info = {"bytes": 2.0 * k.numel() * 2, "flops": 4.0 * B * Hq * D * width * page}
+    elif args.op == "verify_drafts":
+        B, K_, V = 64, 5, 151936
+        p = torch.softmax(torch.randn(B, K_ + 1, V, device=dev) * 2.5, -1)
+        d, u = torch.randint(0, V, (B, K_), device=dev), torch.rand(B, K_ + 1, device=dev)
+        pd = p[:, :K_].contiguous()
+        fn = lambda: ops.verify_drafts(d, p, u, pd)
+        info = {"bytes": 2.0 * B * V * 4}
+    elif args.op == "page_fork":  # a prompt of 1000 tokens, 15 more samples, 16 layers: the copies of its last page
+        from ..models import PagePool
+        pool = PagePool(16, 256, 16, 2048, 8)
+        first = torch.zeros(16, device=dev, dtype=torch.int32)
+        first[0] = 1000
+        pool.reserve(first), pool.advance(first)
+        rows = torch.arange(16, device=dev, dtype=torch.int32)
+
+        def fn():
+            pool.fork(torch.zeros_like(rows[1:]), rows[1:])
+            pool.reserve(1, check=False)
+        info = {"bytes": 2.0 * 15 * (1000 % 64) * 8 * 128 * 2 * 2 * 16}
     else:  # qk_norm_rope
         T, Hq, Hkv, D = 16384, 64, 8, 128
         qkv = torch.randn(T, (Hq + 2 * Hkv) * D, device=dev, dtype=dt)

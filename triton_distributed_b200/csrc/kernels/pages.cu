@@ -16,6 +16,7 @@
 namespace b200 {
 
 constexpr int kPlanThreads = 1024;
+constexpr int kLongRows = 64;
 
 // Inclusive sum over the threads of a CTA of kPlanThreads; `total` is the CTA's. All threads call it.
 __device__ __forceinline__ int block_scan(int v, int* warp_sums, int& total) {
@@ -37,6 +38,12 @@ __device__ __forceinline__ int block_scan(int v, int* warp_sums, int& total) {
   total = __shfl_sync(0xffffffffu, w, 31);
   const int front = __shfl_sync(0xffffffffu, w, max(warp - 1, 0));
   return v + (warp > 0 ? front : 0);
+}
+
+// The counts of pages i ... i + 3, one beyond the last page as `none`.
+__device__ __forceinline__ int4 four_counts(const int* refs, int i, int N, int none) {
+  if (i + 4 <= N && (reinterpret_cast<uintptr_t>(refs) & 15u) == 0) return *reinterpret_cast<const int4*>(refs + i);
+  return make_int4(i < N ? refs[i] : none, i + 1 < N ? refs[i + 1] : none, i + 2 < N ? refs[i + 2] : none, i + 3 < N ? refs[i + 3] : none);
 }
 
 // ---- fork ------------------------------------------------------------------------------------
@@ -137,7 +144,7 @@ __global__ void trim_kernel(int* __restrict__ table, int* __restrict__ lens, int
 struct RowPlan {
   int copy;         // the page that is copied, or -1
   int held, need;   // entries [held, need) are given fresh pages
-  int first;        // the row's first request, by its place among those of the same thread
+  int first;        // the row's first request among all
 };
 struct ReserveParams {
   int* table;
@@ -155,11 +162,11 @@ struct ReserveParams {
 };
 __global__ void __launch_bounds__(kPlanThreads) reserve_plan_kernel(const ReserveParams p) {
   __shared__ int warp_sums[32];
-  __shared__ int s_too_long, s_moves;
+  __shared__ int s_too_long, s_moves, s_n_long, s_long[kLongRows];
   griddep_wait();
   griddep_launch_dependents();
   const int tid = threadIdx.x;
-  if (tid == 0) { s_too_long = 0; s_moves = 0; }
+  if (tid == 0) { s_too_long = 0; s_moves = 0; s_n_long = 0; }
   const int each = (p.R + kPlanThreads - 1) / kPlanThreads;   // thread t plans rows [t * each, (t + 1) * each)
   const int r0 = min(p.R, tid * each), r1 = min(p.R, r0 + each);
   auto entry = [&](int r, int w) -> int& { return p.table[static_cast<size_t>(r) * p.W + w]; };
@@ -182,7 +189,7 @@ __global__ void __launch_bounds__(kPlanThreads) reserve_plan_kernel(const Reserv
   }
   __syncthreads();
   // ---- requests, in the order of the rows ----
-  int sum = 0, total, free_total;
+  int sum = 0, total;
   for (int r = r0; r < r1; ++r) {
     RowPlan plan = p.rows[r];
     const int c = count_of(r), len = max(0, p.lens[r]);
@@ -197,39 +204,63 @@ __global__ void __launch_bounds__(kPlanThreads) reserve_plan_kernel(const Reserv
     p.rows[r] = plan;
   }
   const int before = block_scan(sum, warp_sums, total) - sum;
-  // ---- free pages, in ascending order ----
-  const int per = (p.N + kPlanThreads - 1) / kPlanThreads;
-  const int i0 = min(p.N, tid * per), i1 = min(p.N, i0 + per);
-  int here = 0;
-  for (int i = i0; i < i1; ++i) here += p.refs[i] <= 0;
-  int k = block_scan(here, warp_sums, free_total) - here;
-  const bool fits = s_too_long == 0 && total <= free_total;
-  if (fits)
-    for (int i = i0; i < i1 && k < total; ++i)
-      if (p.refs[i] <= 0) p.fresh[k++] = i;
+  // ---- the lowest free pages, as many as are asked for ----
+  int found = 0;
+  for (int i0 = 0; i0 < p.N && found < total; i0 += 4 * kPlanThreads) {
+    const int i = i0 + 4 * tid;
+    const int4 c = four_counts(p.refs, i, p.N, 1);
+    const int here = (c.x <= 0) + (c.y <= 0) + (c.z <= 0) + (c.w <= 0);
+    int in_tile, k = found + block_scan(here, warp_sums, in_tile) - here;
+    if (c.x <= 0 && k < total) p.fresh[k] = i;
+    k += c.x <= 0;
+    if (c.y <= 0 && k < total) p.fresh[k] = i + 1;
+    k += c.y <= 0;
+    if (c.z <= 0 && k < total) p.fresh[k] = i + 2;
+    k += c.z <= 0;
+    if (c.w <= 0 && k < total) p.fresh[k] = i + 3;
+    found += in_tile;
+  }
+  const bool fits = s_too_long == 0 && total <= found;
   __syncthreads();
   if (fits) {
     for (int r = r0; r < r1; ++r) {
       const RowPlan plan = p.rows[r];
-      int at = before + plan.first;
+      const int first = before + plan.first;
+      p.rows[r].first = first;
       if (plan.copy >= 0) {
-        const int to = p.fresh[at++], len = p.lens[r];
+        const int to = p.fresh[first], len = p.lens[r];
         p.moves[atomicAdd(&s_moves, 1)] = make_int4(plan.copy, to, len % p.page, 0);
         entry(r, len / p.page) = to;
         atomicAdd(p.refs + plan.copy, -1);
         p.refs[to] = 1;
       }
-      for (int w = plan.held; w < plan.need; ++w) {
-        const int to = p.fresh[at++];
+    }
+    __syncthreads();
+    auto give = [&](int r, const RowPlan& plan, int thread, int threads) {
+      const int first = plan.first + (plan.copy >= 0) - plan.held;
+      for (int w = plan.held + thread; w < plan.need; w += threads) {
+        const int to = p.fresh[first + w];
         entry(r, w) = to;
         p.refs[to] = 1;
       }
+    };
+    for (int r = tid >> 5; r < p.R; r += kPlanThreads / 32) {   // a row by a warp; a prompt (as many as are remembered) by the CTA
+      const RowPlan plan = p.rows[r];
+      int place = kLongRows;
+      if (plan.need - plan.held > 256) {
+        if ((tid & 31) == 0) place = atomicAdd(&s_n_long, 1);
+        place = __shfl_sync(0xffffffffu, place, 0);
+      }
+      if (place < kLongRows) s_long[place] = r;
+      else give(r, plan, tid & 31, 32);
     }
+    __syncthreads();
+    for (int i = 0; i < min(s_n_long, kLongRows); ++i) give(s_long[i], p.rows[s_long[i]], tid, kPlanThreads);
   }
   __syncthreads();
   if (tid == 0) {
     *p.n_moves = s_moves;
-    *p.status = s_too_long ? 2 : total > free_total ? 1 : 0;
+    *p.status = s_too_long ? 2 : total > found ? 1 : 0;
   }
 }
 
@@ -250,25 +281,34 @@ __global__ void __launch_bounds__(kPlanThreads) compact_plan_kernel(const Compac
   __shared__ int warp_sums[32];
   griddep_wait();
   griddep_launch_dependents();
-  const int tid = threadIdx.x, per = (p.N + kPlanThreads - 1) / kPlanThreads;
-  const int i0 = min(p.N, tid * per), i1 = min(p.N, i0 + per);
-  int n = 0, live, movers, holes;
-  for (int i = i0; i < i1; ++i) n += p.refs[i] > 0;
-  block_scan(n, warp_sums, live);
-  int moving = 0, hole = 0;
-  for (int i = i0; i < i1; ++i) {
-    const bool used = p.refs[i] > 0;
-    moving += used && i >= live;
-    hole += !used && i < live;
+  const int tid = threadIdx.x;
+  int n = 0, live;
+#pragma unroll 4
+  for (int i = 4 * tid; i < p.N; i += 4 * kPlanThreads) {
+    const int4 c = four_counts(p.refs, i, p.N, 0);
+    n += (c.x > 0) + (c.y > 0) + (c.z > 0) + (c.w > 0);
   }
-  int km = block_scan(moving, warp_sums, movers) - moving, kh = block_scan(hole, warp_sums, holes) - hole;
-  for (int i = i0; i < i1; ++i) {
-    const int count = p.refs[i];
-    const bool used = count > 0;
-    if (used && i >= live) p.from[km++] = i;
-    if (!used && i < live) p.to[kh++] = i;
-    p.remap[i] = i;
-    if (p.refs_out != p.refs) p.refs_out[i] = count;
+  block_scan(n, warp_sums, live);
+  int movers = 0, holes = 0;
+  for (int base = 0; base < p.N; base += 4 * kPlanThreads) {
+    const int i = base + 4 * tid;
+    const int4 c = four_counts(p.refs, i, p.N, i >= live ? 0 : 1);   // (pages that are not there neither move nor are holes)
+    const int count[4] = {c.x, c.y, c.z, c.w};
+    int here = 0, in_tile;   // pages that move, holes << 16
+#pragma unroll
+    for (int e = 0; e < 4; ++e) here += count[e] > 0 && i + e >= live && i + e < p.N ? 1 : count[e] <= 0 && i + e < live ? 1 << 16 : 0;
+    const int front = block_scan(here, warp_sums, in_tile) - here;
+    int km = movers + (front & 0xffff), kh = holes + (front >> 16);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      if (i + e >= p.N) break;
+      if (count[e] > 0 && i + e >= live) p.from[km++] = i + e;
+      if (count[e] <= 0 && i + e < live) p.to[kh++] = i + e;
+      p.remap[i + e] = i + e;
+      if (p.refs_out != p.refs) p.refs_out[i + e] = count[e];
+    }
+    movers += in_tile & 0xffff;
+    holes += in_tile >> 16;
   }
   __syncthreads();
   for (int k = tid; k < movers; k += kPlanThreads) {   // as many holes as movers

@@ -18,7 +18,7 @@
 // weights anew from the scores, which are still there because the weights stay in registers until then. Over a long range the maximum of the first
 // steps stands, so this is rare, and the chain of a step is one pass over the scores instead of two. Weights above one are rounded like those
 // below (relative to themselves); what is lost is that a row's largest weight was held exactly: error against 64 bits 2.3e-3 of the norm before and now.
-// Pages: a step's 128 keys are 128 / page copies (or one, of pages of 128 and more); page numbers are read a window of 32 ahead by
+// Pages: a step's 128 keys are one copy, or 128 / p of p keys, p the largest power of two that divides a page; page numbers are read a window of 32 ahead by
 // the producer's lanes. Pages outside the cache are copies from behind its end, which give zeros.
 // Rows leave their normalised output in fp32 and their log-sum-exp, one range per CTA.
 #include "b200/host.h"
@@ -42,6 +42,11 @@ struct PrefixShape {
   static constexpr int kSmem = kQTiles * kTile + 2 * kStages * kTile + 1024 /*alignment*/ + 256 /*barriers*/ + kXM * 8 /*references and sums of the odd steps*/;
 };
 
+// Keys per copy: the largest power of two that divides a page, so that a copy lies in one page, and steps consist of whole copies.
+__host__ __device__ __forceinline__ int prefix_copy_rows(int page) {
+  const int rows = page & -page;
+  return rows < kXN ? rows : kXN;
+}
 __device__ __forceinline__ float prefix_exp2(float x) {   // one instruction; -inf gives 0
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -129,7 +134,7 @@ shared_prefix_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kXOtherRegs));
     if (warp == 8) {
       // ---------------------------------------------------------------- TMA producer: the warp reads page numbers, every lane copies a part of a step
-      const int rows = min(p.page, kXN), pieces = kXN / rows;   // keys per copy, copies per step
+      const int rows = prefix_copy_rows(p.page), pieces = kXN / rows;   // keys per copy, copies per step
       const int piece0 = key0 / rows, piece_end = (p.shared + rows - 1) / rows;   // copies are numbered from the first key on
       auto page_at = [&](int piece) -> int {   // first slot of a copy (behind the cache's end where there is no such page)
         if (piece >= piece_end) return 0;
@@ -466,10 +471,10 @@ static int launch_prefix(const CUtensorMap& tq, const CUtensorMap& tk, const CUt
   return kOk;
 }
 
-// Whether the kernel handles a call at all: whole groups of query heads in a tile, pages that steps of 128 keys are made of (or that are made of
-// such steps), slots that a 32-bit coordinate reaches.
+// Whether the kernel handles a call at all: whole groups of query heads in a tile, pages of whole swizzle atoms (8 keys), slots that a 32-bit
+// coordinate reaches.
 bool shared_prefix_tc_takes(const SharedPrefixParams& p, int D) {
-  return p.shared > 0 && p.Hq / p.Hkv <= kXM && (D == 64 || D == 128) && p.page >= 8 && (p.page % kXN == 0 || kXN % p.page == 0) &&
+  return p.shared > 0 && p.Hq / p.Hkv <= kXM && (D == 64 || D == 128) && p.page % 8 == 0 &&
          static_cast<long long>(p.num_blocks) * p.page < 0x7fffff00LL && p.Hkv <= 65535;
 }
 
@@ -477,7 +482,7 @@ bool shared_prefix_tc_takes(const SharedPrefixParams& p, int D) {
 int shared_prefix_tc_launch(const SharedPrefixParams& p, int D, int dtype, cudaStream_t s) {
   const int G = p.Hq / p.Hkv, tile_tokens = kXM / G, tiles = (p.B * p.T + tile_tokens - 1) / tile_tokens;
   const bool two_ranges = tiles == 1;
-  const int rows = p.page < kXN ? p.page : kXN;
+  const int rows = prefix_copy_rows(p.page);
   const uint64_t slots = static_cast<uint64_t>(p.num_blocks) * p.page;
   CUtensorMap tq, tk, tv;
   int rc = make_tma_3d(&tq, p.q, dtype, D, p.Hq, static_cast<uint64_t>(p.B) * p.T, D, static_cast<uint64_t>(p.ldq), 64, G, tile_tokens, true);

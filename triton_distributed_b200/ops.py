@@ -1034,7 +1034,7 @@ def choose_prefix_splits(batch: int, tokens: int, heads: int, kv_heads: int, sha
     rows = batch * tokens * group
     blocks = lambda n: -(-n // (8 if n <= 8 else 16 if n <= 16 else 32))  # noqa: E731  (CTAs for n rows of the warp kernel)
     own_ctas = batch * kv_heads * blocks(tokens * group)
-    able = shared > 0 and group <= 128 and page >= 8 and (page % 128 == 0 or 128 % page == 0) and slots < 0x7fffff00 and kv_heads <= 65535
+    able = shared > 0 and group <= 128 and page % 8 == 0 and slots < 0x7fffff00 and kv_heads <= 65535
     if variant == "tc" and not able:
         raise ValueError("shared_prefix_attention: these heads or pages are not for the tensor-core kernel")
     tc = able and (rows > 16 if variant is None else variant == "tc")
@@ -1073,7 +1073,7 @@ def shared_prefix_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: tor
     row of the block table, which has to hold them then) for every sequence that reaches beyond them with all its tokens; shorter sequences (also
     kv_lens 0) are attended over their own table alone. ``shared`` need not be a multiple of the page. ``max_kv_len``: an upper bound on kv_lens for the choice
     of splits (default: what the table can hold). ``variant``: which kernel reads the shared keys, "warp" (warp-level products, any page) or "tc" (tcgen05 tiles; pages
-    that 128 is a multiple of, or that are multiples of 128); None picks by the rows per KV head. Returns [B * tokens, Hq, D] (and the natural-log LSE fp32 [B * tokens, Hq])."""
+    of a multiple of 8); None picks by the rows per KV head. Returns [B * tokens, Hq, D] (and the natural-log LSE fp32 [B * tokens, Hq])."""
     if q.dim() != 3 or k_cache.dim() != 4 or k_cache.shape != v_cache.shape or kv_lens.dim() != 1 or block_table.dim() != 2:
         raise ValueError("shared_prefix_attention: q [B * tokens, Hq, D], caches [num_blocks, page, Hkv, D], kv_lens [B], block_table [B, max_blocks]")
     shared, tokens = int(shared), int(tokens)
@@ -1213,7 +1213,8 @@ def fork_pages(block_table: torch.Tensor, kv_lens: torch.Tensor, refs: torch.Ten
     """Rows ``dst[i]`` of the block table become copies of rows ``src[i]``, in place and without moving data: they let go of what they held
     and hold the pages of the source's tokens (``refs`` counts how many entries hold a page). All sources are read as they were before the
     call, so rows can be exchanged; pairs with a row outside the table and all but the first pair of a destination are skipped. The page that the source's last token is in is shared too:
-    ``reserve_pages`` copies it for whoever writes next. src, dst: whole numbers [n], lists or tensors."""
+    ``reserve_pages`` copies it for whoever writes next. src, dst: whole numbers [n], lists or tensors (lists are copied to the device: not inside a
+    capture)."""
     page_size = int(page_size)
     R, W, N = _check_page_state("fork_pages", block_table, refs, kv_lens, page_size)
     src, dst = _rows("fork_pages", src, block_table.device), _rows("fork_pages", dst, block_table.device)
