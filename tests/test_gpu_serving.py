@@ -99,6 +99,29 @@ def test_keys_that_are_no_numbers(variant):
         assert bool(out[:, 8:][gone].isnan().all()) and bool(out[:, 8:][~gone].isfinite().all())
 
 
+@pytest.mark.parametrize("first,end,value", [(5, 6, float("nan")), (40, 41, float("nan")), (40, 41, float("inf")), (0, 40, float("inf")),
+                                              (0, 128, float("inf")), (128, 256, float("inf")), (0, 1000, float("inf"))])
+@pytest.mark.parametrize("B", [4, 40])
+def test_first_keys_that_are_no_numbers(B, first, end, value):
+    """The first keys give the softmax on the tensor cores its reference: none of them, some, whole steps or all shared keys may have scores of minus
+    infinity (for the other half of the rows plus infinity, which like NaN makes a row NaN)."""
+    from triton_distributed_b200 import ops, ref
+    c = prefix_batch(B, 1, 16, 2, 128, 64, 1000, 40, seed=first + end, device="cuda")
+    page, at = c["block_table"][0].long(), torch.arange(first, end, device="cuda")
+    c["k_cache"][page[at // 64], at % 64, 1, 3] = value
+    want, want_lse = ref.shared_prefix_attention_ref(**c)
+    spread, _ = ref.shared_prefix_attention_ref(**{**c, "v_cache": c["v_cache"].abs()})
+    out, lse = ops.shared_prefix_attention(**c, return_lse=True, variant="tc")
+    ops.check_pipeline_status()
+    s = c["q"][..., 3].float() * value
+    gone = s.isnan() | (s == float("inf"))
+    gone[..., :8] = False                      # the other KV head's keys are numbers
+    assert bool(gone.any()) and bool(out[gone].isnan().all())
+    out, want, spread = (x.masked_fill(gone[..., None], 0) for x in (out, want, spread))
+    lse, want_lse = (x.masked_fill(gone, 0) for x in (lse, want_lse))
+    _check_attention(c, out, lse, want, want_lse, spread)
+
+
 @pytest.mark.parametrize("T,shared", [(1, 200), (4, 200), (3, 64)])
 @pytest.mark.parametrize("B", [6, 150])
 def test_shared_prefix_attention_of_short_rows(T, shared, B):

@@ -13,11 +13,12 @@
 //   warp 9       one elected thread issues tcgen05.mma, for each step and tile O += P V of this step, then S = Q K^T of the next
 // Tensor memory: S of tile t at columns 128 t, O of tile t at 256 + 128 t. P is written over S as 16-bit pairs and is the A operand of
 // the second product; V is read in place as an MN-major B operand.
-// The softmax of a step does not wait for its maximum: the weights are taken against the reference of the steps before, and only if one of
-// a warp's scores lies above it by more than 8 (or at the first step) the warp raises its rows' references to their maxima, rescales their output and takes the step's
-// weights anew from the scores, which are still there because the weights stay in registers until then. Over a long range the maximum of the first
-// steps stands, so this is rare, and the chain of a step is one pass over the scores instead of two. Weights above one are rounded like those
-// below (relative to themselves); what is lost is that a row's largest weight was held exactly: error against 64 bits 2.3e-3 of the norm before and now.
+// The softmax of a step does not wait for its maximum: the weights are taken against the reference of the steps before (at the first step: the maximum
+// of its first 32 keys), and only if one of a warp's scores lies above it by more than 8 the warp raises its rows' references to their maxima, rescales
+// their output and takes the step's weights anew from the scores, which are still there because the weights stay in registers until then. The maximum
+// of the first keys mostly stands, so this is rare, and the chain of a step is one pass over the scores instead of two (two passes at the first step
+// only, for the maximum of all its keys: 18.0 instead of 17.1 us for 16 rows of 64 / 8 heads over 2048 keys). Weights above one are rounded like those
+// below (relative to themselves); what is lost is that a row's largest weight was held exactly: error against 64 bits 2.3e-3 of the norm both ways.
 // Pages: a step's 128 keys are one copy, or 128 / p of p keys, p the largest power of two that divides a page; page numbers are read a window of 32 ahead by
 // the producer's lanes. Pages outside the cache are copies from behind its end, which give zeros.
 // Rows leave their normalised output in fp32 and their log-sum-exp, one range per CTA.
@@ -39,7 +40,7 @@ struct PrefixShape {
   static constexpr int kTile = kAtoms * kXAtom;
   static constexpr int kQTiles = kTwoRanges ? 1 : 2;
   static constexpr int kStages = kTwoRanges ? (kAtoms == 2 ? 3 : 4) : (kAtoms == 2 ? 2 : 4);   // of K, and as many of V
-  static constexpr int kSmem = kQTiles * kTile + 2 * kStages * kTile + 1024 /*alignment*/ + 256 /*barriers*/ + kXM * 8 /*references and sums of the odd steps*/;
+  static constexpr int kSmem = kQTiles * kTile + 2 * kStages * kTile + 1024 /*alignment*/ + 256 /*barriers*/;
 };
 
 // Keys per copy: the largest power of two that divides a page, so that a copy lies in one page, and steps consist of whole copies.
@@ -85,7 +86,6 @@ shared_prefix_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
   uint64_t* o_full = bars + 21;      // [2 tiles] the last product is done
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 23);
   volatile uint32_t* abort_flag = tmem_slot + 1;
-  float2* s_odd = reinterpret_cast<float2*>(bars + 32);    // [128 rows] kTwoRanges: reference and sum of the odd steps
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint64_t timeout_ns = 4000000000ull;
@@ -141,7 +141,6 @@ shared_prefix_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
         const int per_page = p.page / rows, blk = p.prefix_table[piece / per_page];
         return blk >= 0 && blk < p.num_blocks ? blk * p.page + piece % per_page * rows : p.num_blocks * p.page;
       };
-      int window = piece0, now = page_at(piece0 + lane), next = page_at(piece0 + 32 + lane);
       bool ok = true;
       if (lane == 0 && n_steps > 0) {
         int tiles = 0;
@@ -152,6 +151,7 @@ shared_prefix_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
 #pragma unroll
             for (int a = 0; a < kAtoms; ++a) tma_load_3d(sQ + t * kTile + a * kXAtom, &tmQ, q_full, 64 * a, kvh * G, token0_of(t));
       }
+      int window = piece0, now = page_at(piece0 + lane), next = page_at(piece0 + 32 + lane);
       const int piece = lane / kAtoms, atom = lane % kAtoms;   // each lane makes one copy of a step (24 x 5 drafts, pages of 16: 33.5 us, 40 with one lane for all)
       int done = 0;
       for (int j = 0; j < n_steps; ++j) {
@@ -271,6 +271,9 @@ shared_prefix_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
     const uint32_t lanes = tmem_base + (static_cast<uint32_t>((warp & 3) * 32) << 16);
     const uint32_t s_addr = lanes + t * kXN, o_addr = lanes + 2 * kXN + t * 128;
     const int steps = steps_of(t);
+    const int token = token0_of(t) + row / G;
+    const bool mine = row < tile_rows && token < all_tokens;
+    const bool valid = mine && n_steps > 0 && p.kv_lens[token / p.T] - p.T + 1 >= p.shared;   // (else the sequence ends inside the shared keys)
     float ref = -INFINITY, sum = 0.f;   // the row's reference (of scaled scores) and the sum of 2^(score - reference)
     bool ok = true;
     for (int j = 0; j < steps; ++j) {
@@ -301,36 +304,34 @@ shared_prefix_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
         }
       };
       float mx = -INFINITY;   // of the scores; NaN if one of them is
-      bool raise = j == 0;
-      if (j > 0) {
-        sums[0] = sums[1] = pack2(0.f, 0.f);
-        const f32x2 base2 = pack2(-ref, -ref);
+      auto look = [&](const uint32_t (&r)[32]) {
+#pragma unroll
+        for (int e = 0; e < 32; e += 2) mx = max3_nan(mx, __uint_as_float(r[e]), __uint_as_float(r[e + 1]));
+      };
+      sums[0] = sums[1] = pack2(0.f, 0.f);
+      {
         uint32_t r[2][32];
         fetch(0, r[0]);
+        tmem_ld_wait();
+        fetch(1, r[1]);
+        hide_tail(0, r[0]);
+        look(r[0]);
+        if (j == 0) ref = mx * p.scale_log2e;   // the first reference: the maximum of the first keys (none if that is NaN)
+        const f32x2 base2 = pack2(-ref, -ref);
+        weigh(0, r[0], base2);
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
+        for (int c = 1; c < 4; ++c) {
           tmem_ld_wait();
           if (c < 3) fetch(c + 1, r[(c + 1) & 1]);
           hide_tail(c, r[c & 1]);
           weigh(c, r[c & 1], base2);
-#pragma unroll
-          for (int e = 0; e < 32; e += 2) mx = max3_nan(mx, __uint_as_float(r[c & 1][e]), __uint_as_float(r[c & 1][e + 1]));
-        }
-        raise = __any_sync(0xffffffffu, !(mx * p.scale_log2e - ref <= kXRaise));   // (also without a reference, and with NaN)
-      } else {
-#pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          uint32_t r[32];
-          fetch(c, r);
-          tmem_ld_wait();
-          hide_tail(c, r);
-#pragma unroll
-          for (int e = 0; e < 32; e += 2) mx = max3_nan(mx, __uint_as_float(r[e]), __uint_as_float(r[e + 1]));
+          look(r[c & 1]);
         }
       }
+      const bool raise = __any_sync(0xffffffffu, !(mx * p.scale_log2e - ref <= kXRaise));   // (also without a reference, and with NaN)
       if (raise) {
         const float top = fmaxf(ref, mx * p.scale_log2e), base = top == -INFINITY ? 0.f : top;
-        const float corr = ref == -INFINITY ? 0.f : prefix_exp2(ref - base);
+        const float corr = ref == -INFINITY || ref != ref ? 0.f : prefix_exp2(ref - base);
         ref = top;
         sum *= corr;
         if (j > 0) {
@@ -381,47 +382,49 @@ shared_prefix_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
       ok = __all_sync(0xffffffffu, mbar_wait(o_full + t, 0, abort_flag, timeout_ns));
       tc_fence_after_sync();
     }
-    const int token = token0_of(t) + row / G;
-    const bool mine = row < tile_rows && token < all_tokens && (!kTwoRanges || t == 0);
     const size_t range = (static_cast<size_t>(token) * p.Hq + kvh * G + row % G) * p.S + split;
-    float weight = 1.f, weight_odd = 0.f;   // of this tile's output and of the odd steps'
-    // (all products are done: the K ring holds the odd steps' output, row by row, its 16-byte chunks exchanged so that rows lie in all banks)
-    float4* odd = reinterpret_cast<float4*>(sK) + row * (D / 4);
+    float weight = 1.f, weight_other = 0.f;   // of this tile's output and of the other steps'
+    // With two ranges the tiles exchange halves of their columns and each stores one. The K ring holds the halves, row by row, the 16-byte
+    // chunks exchanged so that rows lie in all banks. (A tile's last product is issued after all products of scores, so nothing reads K now.)
+    constexpr int kCols = kTwoRanges ? D / 2 : D, kChunks = D / 8;   // columns that a thread stores; 16-byte chunks of a half row
+    static_assert(!kTwoRanges || 2 * kXM * (kChunks * 16 + 8) <= kSt * kTile, "the K ring holds both tiles' halves, references and sums");
+    const int col0 = kTwoRanges ? t * kCols : 0;
+    float4* other = reinterpret_cast<float4*>(sK) + (t * kXM + row) * kChunks;   // what the other tile left of this tile's columns
+    float2* s_stat = reinterpret_cast<float2*>(sK + 2 * kXM * kChunks * 16);   // [2 tiles][128 rows] references and sums
+    const bool both = kTwoRanges && n_steps > 1;
     if constexpr (kTwoRanges) {
-      const bool has_odd = n_steps > 1;
-      if (t == 1 && has_odd && ok) {
-        s_odd[row] = make_float2(ref, sum);
+      if (both && ok) {
+        float4* left = reinterpret_cast<float4*>(sK) + ((t ^ 1) * kXM + row) * kChunks;
+        s_stat[t * kXM + row] = make_float2(ref, sum);
 #pragma unroll
-        for (int c = 0; c < D / 16; ++c) {
+        for (int c = 0; c < D / 32; ++c) {
           uint32_t o[16];
-          tmem_ld_32x16(o_addr + c * 16, o);
+          tmem_ld_32x16(o_addr + (D / 2 - col0) + c * 16, o);
           tmem_ld_wait();
 #pragma unroll
           for (int q = 0; q < 4; ++q)
-            odd[(c * 4 + q) ^ (row & (D / 4 - 1))] = make_float4(__uint_as_float(o[4 * q]), __uint_as_float(o[4 * q + 1]), __uint_as_float(o[4 * q + 2]),
-                                                                 __uint_as_float(o[4 * q + 3]));
+            left[(c * 4 + q) ^ (row & (kChunks - 1))] = make_float4(__uint_as_float(o[4 * q]), __uint_as_float(o[4 * q + 1]), __uint_as_float(o[4 * q + 2]),
+                                                                    __uint_as_float(o[4 * q + 3]));
         }
       }
       asm volatile("bar.sync 1, 256;" ::: "memory");   // (both tiles' warps get here, after an abort too)
-      if (has_odd && *abort_flag == 0u) {
-        const float2 x = s_odd[row];
+      if (both && *abort_flag == 0u) {
+        const float2 x = s_stat[(t ^ 1) * kXM + row];
         const float top = fmaxf(ref, x.x), base = top == -INFINITY ? 0.f : top;
         weight = prefix_exp2(ref - base);
-        weight_odd = prefix_exp2(x.x - base);
-        sum = sum * weight + x.y * weight_odd;
+        weight_other = prefix_exp2(x.x - base);
+        sum = sum * weight + x.y * weight_other;
         ref = top;
       }
     }
-    if (ok && mine) {
-      if (steps == 0 || p.kv_lens[token / p.T] - p.T + 1 < p.shared) p.lse_part[range] = -INFINITY;   // (the sequence ends inside the shared keys)
-      else p.lse_part[range] = (ref + log2f(sum)) * 0.6931471805599453f;
-    }
-    if (ok && steps > 0 && !(kTwoRanges && t == 1)) {
-      const bool valid = mine && p.kv_lens[token / p.T] - p.T + 1 >= p.shared;
+    const bool stores = ok && (kTwoRanges ? both || t == 0 : true);   // (with one step the first tile has all columns)
+    if (stores && mine && (!kTwoRanges || t == 0)) p.lse_part[range] = valid && steps > 0 ? (ref + log2f(sum)) * 0.6931471805599453f : -INFINITY;
+    if (stores && steps > 0) {
       const float inv = 1.f / sum;
 #pragma unroll
       for (int c = 0; c < D / 16; ++c) {
-        const int col = c * 16;
+        if (kTwoRanges && c >= kCols / 16 && both) break;
+        const int col = (kTwoRanges && !both ? 0 : col0) + c * 16;
         uint32_t o[16];
         tmem_ld_32x16(o_addr + col, o);
         tmem_ld_wait();
@@ -430,11 +433,11 @@ shared_prefix_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
           float v[8];
 #pragma unroll
           for (int e = 0; e < 8; ++e) v[e] = __uint_as_float(o[q * 8 + e]) * weight;
-          if (kTwoRanges && n_steps > 1) {
+          if (both) {
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-              const float4 x = odd[(col / 4 + q * 2 + h) ^ (row & (D / 4 - 1))];
-              v[4 * h] += x.x * weight_odd; v[4 * h + 1] += x.y * weight_odd; v[4 * h + 2] += x.z * weight_odd; v[4 * h + 3] += x.w * weight_odd;
+              const float4 x = other[(c * 4 + q * 2 + h) ^ (row & (kChunks - 1))];
+              v[4 * h] += x.x * weight_other; v[4 * h + 1] += x.y * weight_other; v[4 * h + 2] += x.z * weight_other; v[4 * h + 3] += x.w * weight_other;
             }
           }
 #pragma unroll
