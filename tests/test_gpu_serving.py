@@ -64,6 +64,25 @@ def test_shared_prefix_attention_tiles(B, T, Hq, Hkv, D, page, shared):
     _attention_case(prefix_batch(B, T, Hq, Hkv, D, page, shared, 20, seed=B, device="cuda"), variant="tc")
 
 
+@pytest.mark.parametrize("B,Hq,Hkv,page,shared,own", [
+    (80, 8, 2, 16, 1000, 5000),     # thousands of own keys for one CTA
+    (80, 2, 2, 48, 999, 4700),
+    (2, 16, 16, 32, 70001, 30),     # of shared ones
+    (1, 16, 16, 24, 50000, 2),      # pages that no slice is made of
+])
+def test_shared_prefix_attention_of_many_keys_for_one_cta(B, Hq, Hkv, page, shared, own):
+    _attention_case(prefix_batch(B, 1, Hq, Hkv, 64, page, shared, own, seed=page, device="cuda"), variant="warp")
+
+
+@pytest.mark.parametrize("kv_lens", [[3, 700], [0, 64], [63, 65], [1, 1], [2048, 2049]])
+@pytest.mark.parametrize("page", [16, 64, 80])
+def test_sequences_that_end_before_the_shared_keys_do(kv_lens, page):
+    """Short sequences beside ones that reach beyond the shared keys: whose first pages are read depends on the length."""
+    for B in (2, 24):
+        lens = (kv_lens * B)[:B]
+        _attention_case(prefix_batch(B, 1, 8, 2, 64, page, 64, 2100, seed=B, lens=lens, device="cuda"))
+
+
 @pytest.mark.parametrize("variant", ["warp", "tc"])
 @pytest.mark.parametrize("B", [3, 40])
 @pytest.mark.parametrize("order", [1, -1, 0])

@@ -66,11 +66,19 @@ __device__ __forceinline__ bool slice_has_nonfinite(uint32_t vs, int lane) {
   return __any_sync(0xffffffffu, bad != 0u);
 }
 
+// Where the slice of keys from token `tok` on (a multiple of 16) begins in the cache, in slices; -1: nowhere. (Pages of a multiple of 16 keys.)
+__device__ __forceinline__ int span_slice_at(const SharedPrefixParams& p, const int* table, int width, unsigned tok) {
+  const unsigned w = tok / p.page;
+  const int blk = w < static_cast<unsigned>(width) ? table[w] : -1;
+  return blk >= 0 && blk < p.num_blocks ? blk * (p.page / kSpanSlice) + static_cast<int>(tok % p.page) / kSpanSlice : -1;
+}
+
 // One CTA: 8 NB rows of KV head `kvh` from row `row0` of a group of `rows`, over keys [t0, t1) of the pages in `table`. A row r of
 // the group is query token first_token + r / G, head kvh * G + r % G. `own`: the rows are one sequence's and see keys below `limit0` + r / G.
+// `ahead`: this lane's span_slice_at of slice warp + 4 * lane counted from key `ahead_base` on, where that has been read already.
 template <bool BF16, int D, int NB>
 __device__ __forceinline__ void span_body(const SharedPrefixParams& p, uint8_t* smem, int kvh, int first_token, int row0, int rows, const int* table,
-                                          int width, int t0, int t1, bool own, int limit0, int split) {
+                                          int width, int t0, int t1, bool own, int limit0, int split, int ahead_base, int ahead) {
   constexpr int kKK = D / 16, kRowBytes = D * 2, kChunks = D / 8, kSliceBytes = kSpanSlice * kRowBytes;
   constexpr int kLaneRows = 32 / kChunks;                  // keys that a warp copies with one instruction
   constexpr int kCopies = kSpanSlice / kLaneRows;
@@ -102,22 +110,28 @@ __device__ __forceinline__ void span_body(const SharedPrefixParams& p, uint8_t* 
   const int hi = lane / kChunks, chunk = lane % kChunks;
   const size_t token_bytes = static_cast<size_t>(p.Hkv) * kRowBytes, step = token_bytes * kLaneRows;
   const size_t lane_off = hi * token_bytes + static_cast<size_t>(kvh) * kRowBytes + chunk * 16;
-  int next_blk = page_fast && mine > 0 ? page_of(base + warp * kSpanSlice) : 0;   // one slice ahead of its copies
+  // lane i knows where slices i and i + 32 of a window of this warp's slices begin
+  auto slice_at = [&](int j) { return span_slice_at(p, table, width, static_cast<unsigned>(base) + (warp + 4 * (j + lane)) * kSpanSlice); };
+  int window = !page_fast ? 0 : base == ahead_base ? ahead : slice_at(0);
+  int next = page_fast && mine > 32 ? slice_at(32) : 0;
   auto load_slice = [&](int j) {   // always commits a group, so that the counting stays uniform
     if (j < mine) {
       const int st0 = base + (warp + 4 * j) * kSpanSlice;
       const uint32_t slot = ring + (j % kSpanRing) * (2 * kSliceBytes);
-      const int blk = next_blk;
-      if (page_fast && j + 1 < mine) next_blk = page_of(st0 + 4 * kSpanSlice);
       if (page_fast) {
-        const bool all = blk >= 0 && st0 >= t0 && st0 + kSpanSlice <= t1;
-        const size_t off = (static_cast<size_t>(max(blk, 0)) * p.page + st0 % p.page) * token_bytes + lane_off;
+        if (j > 0 && j % 32 == 0) {
+          window = next;
+          if (j + 32 < mine) next = slice_at(j + 32);
+        }
+        const int at_slice = __shfl_sync(0xffffffffu, window, j % 32);
+        const bool all = at_slice >= 0 && st0 >= t0 && st0 + kSpanSlice <= t1;
+        const size_t off = static_cast<size_t>(max(at_slice, 0)) * (kSpanSlice * token_bytes) + lane_off;
         const uint8_t *ks = kc + off, *vs = vc + off;
 #pragma unroll
         for (int i = 0; i < kCopies; ++i) {
           const int tok_in = i * kLaneRows + hi, tok = st0 + tok_in;
           const uint32_t at = slot + tok_in * kRowBytes + ((chunk ^ (tok_in & 7)) * 16);
-          const int bytes = all || (blk >= 0 && tok >= t0 && tok < t1) ? 16 : 0;   // (the address is inside the page either way)
+          const int bytes = all || (at_slice >= 0 && tok >= t0 && tok < t1) ? 16 : 0;   // (the address is inside the page either way)
           cp_async_16(at, ks + i * step, bytes);
           cp_async_16(at + kSliceBytes, vs + i * step, bytes);
         }
@@ -342,7 +356,7 @@ __global__ void __launch_bounds__(kSpanThreads) shared_prefix_span_kernel(const 
       const int groups = p.prefix_ctas / p.prefix_splits / p.Hkv;
       const int kvh = at / groups, group = at % groups;
       const int t0 = split * p.prefix_chunk, t1 = min(p.shared, t0 + p.prefix_chunk);
-      span_body<BF16, D, NBP>(p, smem, kvh, 0, group * NBP * 8, p.B * p.T * G, p.prefix_table, (p.shared + p.page - 1) / p.page, t0, t1, false, 0, split);
+      span_body<BF16, D, NBP>(p, smem, kvh, 0, group * NBP * 8, p.B * p.T * G, p.prefix_table, (p.shared + p.page - 1) / p.page, t0, t1, false, 0, split, -1, 0);
       // rows of sequences that do not reach beyond the shared keys are attended by themselves
       __syncthreads();
       for (int r = threadIdx.x; r < NBP * 8; r += kSpanThreads) {
@@ -361,12 +375,20 @@ __global__ void __launch_bounds__(kSpanThreads) shared_prefix_span_kernel(const 
   const int group = at % groups;
   at /= groups;
   const int kvh = at % p.Hkv, b = at / p.Hkv;
-  const int len = max(0, p.kv_lens[b]), start = len - p.T + 1 >= p.shared ? p.shared : 0;
+  const int* table = p.block_table + static_cast<size_t>(b) * p.bt_stride;
+  const int kv_len = p.kv_lens[b];
+  // The first pages as they are for a sequence that reaches beyond the shared keys: read together with its length, not after it. (With a window of 32
+  // page numbers a warp instead of one ahead, and the merge's outputs fetched before its weights: 2 sequences of 32 / 8 heads, 1000 + 64 keys 8.8 ->
+  // 6.9 us; 16 of 64 / 8 heads, 2048 + 512 17.0 -> 14.6; 48 x 3 tokens of 14 / 2 heads of 64, 16384 + 700 33.7 -> 29.0.)
+  const bool known = p.own_splits == 1 && p.page % kSpanSlice == 0;
+  const int ahead_base = known ? p.shared & ~(kSpanSlice - 1) : -1;
+  const int ahead = known ? span_slice_at(p, table, p.width, static_cast<unsigned>(ahead_base) + ((threadIdx.x >> 5) + 4 * (threadIdx.x & 31)) * kSpanSlice) : 0;
+  const int len = max(0, kv_len), start = len - p.T + 1 >= p.shared ? p.shared : 0;
   int chunk = (len - start + p.own_splits - 1) / p.own_splits;
   chunk = (chunk + 4 * kSpanSlice - 1) / (4 * kSpanSlice) * (4 * kSpanSlice);
   const int t0 = start + split * chunk, t1 = min(len, t0 + chunk);
-  span_body<BF16, D, NBO>(p, smem, kvh, b * p.T, group * NBO * 8, rows, p.block_table + static_cast<size_t>(b) * p.bt_stride, p.width, t0, t1,
-                          true, len - p.T + 1, p.prefix_splits + split);
+  span_body<BF16, D, NBO>(p, smem, kvh, b * p.T, group * NBO * 8, rows, table, p.width, t0, t1, true, len - p.T + 1, p.prefix_splits + split,
+                          ahead_base, ahead);
   // The kernel in front (the shared keys') has to be complete before this one is. One CTA sees to that: if all of them waited, they would keep the
   // SMs that the kernel in front leaves free (64 / 8 heads, batch 64, with 64 CTAs in front: 155 us for 130).
   if (p.late_wait && blockIdx.x == gridDim.x - 1) griddep_wait();
@@ -381,29 +403,44 @@ __global__ void __launch_bounds__(128) shared_prefix_merge_kernel(const float* _
   const int row = blockIdx.x * 4 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
   if (row >= rows) return;
   const float* l_row = lse_part + static_cast<size_t>(row) * S;
-  const float* o_row = o_part + static_cast<size_t>(row) * S * D;
-  constexpr int kV = D / 32;   // columns per lane
-  float top = -INFINITY;
-  for (int s = lane; s < S; s += 32) top = fmaxf(top, l_row[s]);
+  constexpr int kV = D / 32, kAhead = 8;   // columns per lane; ranges in flight while those before are added
+  const float* o_row = o_part + static_cast<size_t>(row) * S * D + lane * kV;
+  float v[2][kAhead][kV];
+  auto fetch = [&](int s0, float (&x)[kAhead][kV]) {   // (an empty range has left nothing there: read, but not used)
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i)
+      if (s0 + i < S) {
+        const float* src = o_row + static_cast<size_t>(s0 + i) * D;
+        if (kV == 4) *reinterpret_cast<float4*>(x[i]) = *reinterpret_cast<const float4*>(src);
+        else *reinterpret_cast<float2*>(x[i]) = *reinterpret_cast<const float2*>(src);
+      }
+  };
+  fetch(0, v[0]);
+  float l = lane < S ? l_row[lane] : -INFINITY;
+  float top = l;
+  for (int s = lane + 32; s < S; s += 32) top = fmaxf(top, l_row[s]);
 #pragma unroll
   for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
   const float ref = top == -INFINITY ? 0.f : top;
-  float acc[kV] = {0.f}, den = 0.f;
-  for (int s0 = 0; s0 < S; s0 += 32) {
-    const float l = s0 + lane < S ? l_row[s0 + lane] : -INFINITY;
-    const float mine = l == -INFINITY ? 0.f : expf(l - ref);
-    const int n = min(32, S - s0);
-#pragma unroll 8
-    for (int s = 0; s < n; ++s) {
-      const float w = __shfl_sync(0xffffffffu, mine, s);
-      float v[kV];
-      const float* src = o_row + static_cast<size_t>(s0 + s) * D + lane * kV;
-      if (kV == 4) *reinterpret_cast<float4*>(v) = *reinterpret_cast<const float4*>(src);
-      else *reinterpret_cast<float2*>(v) = *reinterpret_cast<const float2*>(src);
-      den += w;
-      if (w != 0.f)   // an empty range has left nothing there
+  float acc[kV] = {0.f}, den = 0.f, mine = 0.f;
+  for (int s0 = 0; s0 < S; s0 += 2 * kAhead) {
+    if (s0 % 32 == 0) {
+      if (s0 > 0) l = s0 + lane < S ? l_row[s0 + lane] : -INFINITY;
+      mine = l == -INFINITY ? 0.f : expf(l - ref);   // the weight of range s0 + lane
+    }
 #pragma unroll
-        for (int e = 0; e < kV; ++e) acc[e] += w * v[e];
+    for (int half = 0; half < 2; ++half) {
+      const int s1 = s0 + half * kAhead;
+      if (s1 + kAhead < S) fetch(s1 + kAhead, v[half ^ 1]);
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i) {
+        const float w = __shfl_sync(0xffffffffu, mine, (s1 + i) % 32);
+        if (s1 + i < S && w != 0.f) {
+          den += w;
+#pragma unroll
+          for (int e = 0; e < kV; ++e) acc[e] += w * v[half][i][e];
+        }
+      }
     }
   }
   T* dst = out + static_cast<size_t>(row) * D + lane * kV;
