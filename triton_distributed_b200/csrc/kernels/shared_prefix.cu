@@ -37,7 +37,7 @@ constexpr int kSpanMostRows = 32;   // per CTA
 template <int D>
 constexpr int span_smem() {         // the rings; in the end the four warps' maxima, sums and outputs (rows D + 4 floats apart)
   constexpr int rings = 4 * kSpanRing * 2 * kSpanSlice * D * 2, merge = 4 * kSpanMostRows * (2 + D + 4) * 4;
-  return rings > merge ? rings : merge;
+  return (rings > merge ? rings : merge) + kSpanMostRows * D * 2 /*queries*/;
 }
 
 __device__ __forceinline__ float span_exp2(float x) {   // one instruction; -inf gives 0
@@ -66,6 +66,24 @@ __device__ __forceinline__ bool slice_has_nonfinite(uint32_t vs, int lane) {
   return __any_sync(0xffffffffu, bad != 0u);
 }
 
+// The queries of a CTA's rows (row r: query token first_token + (row0 + r) / G) to shared memory: 16-byte chunk c of row r lies at chunk c ^ (r & 7).
+// Rows that do not exist are zero. Commits a group.
+template <int D, int NB>
+__device__ __forceinline__ void span_fetch_queries(const SharedPrefixParams& p, uint8_t* smem, int kvh, int first_token, int row0, int nrows) {
+  constexpr int kChunks = D / 8, kLaneRows = 32 / kChunks;
+  const uint32_t qs = static_cast<uint32_t>(__cvta_generic_to_shared(smem)) + span_smem<D>() - kSpanMostRows * D * 2;
+  const int G = p.Hq / p.Hkv, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int g = row0 + min(lane, nrows - 1);   // lane r knows where row r lies
+  const long long at = (static_cast<long long>(first_token + g / G) * p.ldq + static_cast<long long>(kvh * G + g % G) * D) * 2;
+#pragma unroll
+  for (int r0 = 0; r0 < NB * 8; r0 += 4 * kLaneRows) {
+    const int r = r0 + warp * kLaneRows + lane / kChunks, chunk = lane % kChunks;
+    const long long row_at = __shfl_sync(0xffffffffu, at, r & 31);
+    if (r < NB * 8) cp_async_16(qs + r * D * 2 + ((chunk ^ (r & 7)) * 16), static_cast<const uint8_t*>(p.q) + row_at + chunk * 16, r < nrows ? 16 : 0);
+  }
+  cp_async_commit();
+}
+
 // Where the slice of keys from token `tok` on (a multiple of 16) begins in the cache, in slices; -1: nowhere. (Pages of a multiple of 16 keys.)
 __device__ __forceinline__ int span_slice_at(const SharedPrefixParams& p, const int* table, int width, unsigned tok) {
   const unsigned w = tok / p.page;
@@ -75,7 +93,7 @@ __device__ __forceinline__ int span_slice_at(const SharedPrefixParams& p, const 
 
 // One CTA: 8 NB rows of KV head `kvh` from row `row0` of a group of `rows`, over keys [t0, t1) of the pages in `table`. A row r of
 // the group is query token first_token + r / G, head kvh * G + r % G. `own`: the rows are one sequence's and see keys below `limit0` + r / G.
-// `ahead`: this lane's span_slice_at of slice warp + 4 * lane counted from key `ahead_base` on, where that has been read already.
+// The rows' queries are on their way (span_fetch_queries). `ahead`: this lane's span_slice_at of slice warp + 4 * lane counted from key `ahead_base` on, where that has been read already.
 template <bool BF16, int D, int NB>
 __device__ __forceinline__ void span_body(const SharedPrefixParams& p, uint8_t* smem, int kvh, int first_token, int row0, int rows, const int* table,
                                           int width, int t0, int t1, bool own, int limit0, int split, int ahead_base, int ahead) {
@@ -91,6 +109,7 @@ __device__ __forceinline__ void span_body(const SharedPrefixParams& p, uint8_t* 
     return static_cast<size_t>(first_token + g / G) * p.Hq + kvh * G + g % G;
   };
   if (t0 >= t1) {
+    cp_async_wait<0>();
     for (int r = threadIdx.x; r < nrows; r += kSpanThreads) p.lse_part[row_id(r) * p.S + split] = -INFINITY;
     return;
   }
@@ -152,20 +171,17 @@ __device__ __forceinline__ void span_body(const SharedPrefixParams& p, uint8_t* 
 #pragma unroll
   for (int j = 0; j < kSpanRing - 1; ++j) load_slice(j);
 
-  // ---- Q^T fragments: row nb * 8 + lane / 4, elements 16 kk + col, + 1 and eight further; rows that do not exist are zero ----
+  // ---- Q^T fragments: row nb * 8 + lane / 4, elements 16 kk + col, + 1 and eight further ----
   uint32_t qb[NB][kKK][2];
+  cp_async_wait<kSpanRing - 1>();   // (all groups but the slices')
+  __syncthreads();
+  const uint32_t qs = static_cast<uint32_t>(__cvta_generic_to_shared(smem)) + span_smem<D>() - kSpanMostRows * kRowBytes;
 #pragma unroll
-  for (int nb = 0; nb < NB; ++nb) {
-    const int g = row0 + nb * 8 + row;
-    const bool in = nb * 8 + row < nrows;
-    const uint32_t* src = reinterpret_cast<const uint32_t*>(static_cast<const uint8_t*>(p.q) + (static_cast<size_t>(first_token + g / G) * p.ldq +
-                                                            static_cast<size_t>(kvh * G + g % G) * D) * 2) + (lane & 3);
+  for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
-    for (int kk = 0; kk < kKK; ++kk) {
-      qb[nb][kk][0] = in ? src[kk * 8] : 0u;
-      qb[nb][kk][1] = in ? src[kk * 8 + 4] : 0u;
-    }
-  }
+    for (int kk = 0; kk < kKK; kk += 2)
+      ldmatrix_x4(qs + (nb * 8 + (lane & 7)) * kRowBytes + (((2 * kk + (lane >> 3)) ^ (lane & 7)) * 16), qb[nb][kk][0], qb[nb][kk][1], qb[nb][kk + 1][0],
+                  qb[nb][kk + 1][1]);
   int limit[NB][2];   // of rows nb * 8 + col, + 1
 #pragma unroll
   for (int nb = 0; nb < NB; ++nb)
@@ -317,10 +333,13 @@ __device__ __forceinline__ void span_body(const SharedPrefixParams& p, uint8_t* 
       }
     }
   __syncthreads();
-  constexpr int kVecs = D / 4;
-#pragma unroll 4
-  for (int i = threadIdx.x; i < nrows * kVecs; i += kSpanThreads) {
-    const int r = i / kVecs, c = i - r * kVecs;
+  constexpr int kVecs = D / 4, kWarpRows = 32 / kVecs;
+  const long long my_id = static_cast<long long>(row_id(min(lane, nrows - 1)));   // lane r knows where row r goes
+#pragma unroll 2
+  for (int r0 = warp * kWarpRows; r0 < nrows; r0 += 4 * kWarpRows) {
+    const int r = r0 + lane / kVecs, c = lane % kVecs;
+    const size_t id = static_cast<size_t>(__shfl_sync(0xffffffffu, my_id, r & 31)) * p.S + split;
+    if (r >= nrows) continue;
     float top = -INFINITY;
 #pragma unroll
     for (int w = 0; w < 4; ++w) top = fmaxf(top, red_m[w * kRows + r]);
@@ -333,7 +352,6 @@ __device__ __forceinline__ void span_body(const SharedPrefixParams& p, uint8_t* 
       l += red_l[w * kRows + r] * f;
       o.x += x.x * f; o.y += x.y * f; o.z += x.z * f; o.w += x.w * f;
     }
-    const size_t id = row_id(r) * p.S + split;
     const float inv = l > 0.f ? 1.f / l : (l == l ? 0.f : l);
     *reinterpret_cast<float4*>(p.o_part + id * D + c * 4) = make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
     if (c == 0) p.lse_part[id] = l > 0.f ? top * 0.6931471805599453f + logf(l) : (l == l ? -INFINITY : l);
@@ -356,6 +374,7 @@ __global__ void __launch_bounds__(kSpanThreads) shared_prefix_span_kernel(const 
       const int groups = p.prefix_ctas / p.prefix_splits / p.Hkv;
       const int kvh = at / groups, group = at % groups;
       const int t0 = split * p.prefix_chunk, t1 = min(p.shared, t0 + p.prefix_chunk);
+      span_fetch_queries<D, NBP>(p, smem, kvh, 0, group * NBP * 8, min(NBP * 8, p.B * p.T * G - group * NBP * 8));
       span_body<BF16, D, NBP>(p, smem, kvh, 0, group * NBP * 8, p.B * p.T * G, p.prefix_table, (p.shared + p.page - 1) / p.page, t0, t1, false, 0, split, -1, 0);
       // rows of sequences that do not reach beyond the shared keys are attended by themselves
       __syncthreads();
@@ -375,6 +394,7 @@ __global__ void __launch_bounds__(kSpanThreads) shared_prefix_span_kernel(const 
   const int group = at % groups;
   at /= groups;
   const int kvh = at % p.Hkv, b = at / p.Hkv;
+  span_fetch_queries<D, NBO>(p, smem, kvh, b * p.T, group * NBO * 8, min(NBO * 8, rows - group * NBO * 8));
   const int* table = p.block_table + static_cast<size_t>(b) * p.bt_stride;
   const int kv_len = p.kv_lens[b];
   // The first pages as they are for a sequence that reaches beyond the shared keys: read together with its length, not after it. (With a window of 32
