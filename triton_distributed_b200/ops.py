@@ -1024,8 +1024,9 @@ def choose_prefix_splits(batch: int, tokens: int, heads: int, kv_heads: int, sha
                          dim: int = 128, sm_count: int = 148, variant: str | None = None) -> tuple[bool, int, int]:
     """(tensor-core kernel for the shared keys, ranges of the shared keys, ranges of everybody's own keys) for `shared_prefix_attention`.
 
-    The tensor-core kernel from 17 rows per KV head on (us, warp and tensor-core kernel, 64 / 8 heads of 128, 2048 and 65536 keys: 16 rows 12.1 and 14.0,
-    55.6 and 58.2; 24 rows 15.6 and 14.0, 78.4 and 57.8; 64 rows 17.7 and 14.0, 220 and 59; 14 / 2 heads of 64, 21 rows: 10.2 and 11.2, 35.3 and 24.3).
+    The tensor-core kernel from 17 rows per KV head on (us, warp and tensor-core kernel, 64 / 8 heads of 128, 2048 and 65536 keys: 16 rows 8.5 and 10.0,
+    51.1 and 51.5; 24 rows 11.5 and 10.4, 68.4 and 52.0; 64 rows 15.7 and 10.8, 140 and 53.7; 14 / 2 heads of 64, 14 rows: 6.9 and 8.6, 17.9 and 18.4;
+    21 rows: 8.4 and 8.7, 26.8 and 18.5).
     Warp kernel: one wave of two CTAs per SM, ranges of at least 128 keys. Tensor-core kernel: the number of ranges with the least
     estimated time, from what was measured: a step of 128 keys, a CTA's start and end (6 us), the partial results of one more range (written and read
     at 3 TB/s), and the own keys' CTAs (5 us and 18 ns a key), which run on the SMs that the shared keys leave and behind them. Own keys are split only
