@@ -307,6 +307,19 @@ def test_fork_exchanges_rows():
     ops.fork_pages(table, lens, refs, [], [], 4)
 
 
+@pytest.mark.parametrize("more", [0, 300])
+def test_fork_pairs_outside_the_table_do_not_count(more):
+    """A pair whose source is outside the table is as if it were not there: the next one of its destination counts. (Few pairs, and many.)"""
+    from triton_distributed_b200 import ops, ref
+    table, lens, refs = page_state(9, 5, 60, 4, 3)
+    src, dst = [-1] * more + [-1, 3, 9, 2, 4, 5], [8] * more + [0, 0, 1, 1, 1, -1]
+    want = ref.fork_pages_ref(table, lens, refs, src, dst, 4)
+    assert not torch.equal(want[0], table)
+    got = [t.cuda() for t in (table, lens, refs)]
+    ops.fork_pages(*got, src, dst, 4)
+    _same(got, want)
+
+
 @pytest.mark.parametrize("R,W,N,page", PAGES)
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32, torch.uint8])
 def test_reserve_pages(R, W, N, page, dtype):

@@ -58,7 +58,7 @@ __global__ void fork_stage_kernel(const int* __restrict__ table, const int* __re
   if (threadIdx.x == 0) again = 0;
   __syncthreads();
   for (int j = threadIdx.x; j < i; j += blockDim.x)
-    if (dst[j] == d) again = 1;   // of several pairs with one destination the first counts
+    if (dst[j] == d && src[j] >= 0 && src[j] < R) again = 1;   // of several pairs with one destination the first one inside the table counts
   __syncthreads();
   if (again || s < 0 || s >= R || d < 0 || d >= R) {
     if (threadIdx.x == 0) staged_len[i] = -1;
@@ -95,7 +95,7 @@ __global__ void __launch_bounds__(kPlanThreads) fork_few_kernel(int* table, int*
   for (int i = threadIdx.x; i < n; i += kPlanThreads) {
     const int s = src[i], d = dst[i];
     bool ok = s >= 0 && s < R && d >= 0 && d < R;
-    for (int j = 0; j < i && ok; ++j) ok = dst[j] != d;   // of several pairs with one destination the first counts
+    for (int j = 0; j < i && ok; ++j) ok = dst[j] != d || src[j] < 0 || src[j] >= R;   // of several pairs with one destination the first one inside the table counts
     s_len[i] = ok ? max(0, lens[s]) : -1;
   }
   __syncthreads();
@@ -433,8 +433,8 @@ static int move_pages(MoveParams p, const PageTensor* tensors, int n_tensors, lo
 using namespace b200;
 
 // Rows dst[i] become copies of rows src[i] (int32 [n] on the device; all sources are read as they were before the call): they let go of
-// their pages and hold the ceil(len / page) first ones of the source. Pairs out of range, and all but the first pair of a destination, are
-// skipped. scratch: int32 [n * (W + 1)]; unused, and may be null, for at most 256 pairs and 8192 entries (n * W).
+// their pages and hold the ceil(len / page) first ones of the source. Pairs out of range are skipped, and of the others all but the first of a
+// destination. scratch: int32 [n * (W + 1)]; unused, and may be null, for at most 256 pairs and 8192 entries (n * W).
 B200_API int b200_fork_pages(int* table, int* lens, int* refs, const int* src, const int* dst, int n, int R, int W, int N, int page, int* scratch,
                              void* stream) {
   B200_REQUIRE(n >= 0 && R >= 1 && W >= 1 && N >= 1 && page >= 1, "fork_pages: bad sizes");

@@ -1213,7 +1213,7 @@ def _rows(name: str, rows, device) -> torch.Tensor:
 def fork_pages(block_table: torch.Tensor, kv_lens: torch.Tensor, refs: torch.Tensor, src, dst, page_size: int) -> None:
     """Rows ``dst[i]`` of the block table become copies of rows ``src[i]``, in place and without moving data: they let go of what they held
     and hold the pages of the source's tokens (``refs`` counts how many entries hold a page). All sources are read as they were before the
-    call, so rows can be exchanged; pairs with a row outside the table and all but the first pair of a destination are skipped. The page that the source's last token is in is shared too:
+    call, so rows can be exchanged; pairs with a row outside the table are skipped, and of the others all but the first of a destination. The page that the source's last token is in is shared too:
     ``reserve_pages`` copies it for whoever writes next. src, dst: whole numbers [n], lists or tensors (lists are copied to the device: not inside a
     capture)."""
     page_size = int(page_size)
