@@ -320,6 +320,24 @@ def test_fork_pairs_outside_the_table_do_not_count(more):
     _same(got, want)
 
 
+def test_lengths_that_no_table_holds():
+    """The largest int32 as a length of a row, and as a length to keep: all pages of the table, and nothing outside it is touched."""
+    from triton_distributed_b200 import ops, ref
+    most = 2**31 - 1
+    table, lens, refs = page_state(9, 5, 60, 4, 3)
+    lens[4] = most
+    got = [t.cuda() for t in (table, lens, refs)]
+    want = ref.fork_pages_ref(table, lens, refs, [4, 5], [0, 1], 4)
+    ops.fork_pages(*got, [4, 5], [0, 1], 4)
+    _same(got, want)
+    keep = torch.tensor([most, most, 7, -1, most - 1, most, 3, 0, most], dtype=torch.int32)
+    want = ref.trim_pages_ref(*want, 4, keep)
+    ops.trim_pages(*got, 4, keep.cuda())
+    _same(got, want)
+    assert int(ops.reserve_pages(*got, 1, [torch.zeros(60, 4, 1, device="cuda")])) == 2
+    _same(got, want)
+
+
 @pytest.mark.parametrize("R,W,N,page", PAGES)
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32, torch.uint8])
 def test_reserve_pages(R, W, N, page, dtype):

@@ -47,6 +47,8 @@ __device__ __forceinline__ int4 four_counts(const int* refs, int i, int N, int n
 }
 
 // ---- fork ------------------------------------------------------------------------------------
+__device__ __forceinline__ int pages_of(int len, int page) { return len / page + (len % page != 0); }   // (any length, also one that no table holds)
+
 // A CTA per pair: the new row i in `staged` [n, W] and its length (-1: the pair is skipped), the counts of what is taken and let go. The table is only
 // read here, so that a row may be both a source and a destination (every pair sees the table as it was).
 __global__ void fork_stage_kernel(const int* __restrict__ table, const int* __restrict__ lens, int* refs, const int* __restrict__ src,
@@ -64,7 +66,7 @@ __global__ void fork_stage_kernel(const int* __restrict__ table, const int* __re
     if (threadIdx.x == 0) staged_len[i] = -1;
     return;
   }
-  const int len = max(0, lens[s]), held = (len + page - 1) / page;
+  const int len = max(0, lens[s]), held = pages_of(len, page);
   for (int w = threadIdx.x; w < W; w += blockDim.x) {
     const int old = table[static_cast<size_t>(d) * W + w];
     if (old >= 0 && old < N) atomicAdd(refs + old, -1);
@@ -102,7 +104,7 @@ __global__ void __launch_bounds__(kPlanThreads) fork_few_kernel(int* table, int*
   for (int e = threadIdx.x; e < n * W; e += kPlanThreads) {
     const int i = e / W, w = e - i * W, len = s_len[i];
     if (len < 0) continue;
-    const int old = table[static_cast<size_t>(dst[i]) * W + w], take = w < (len + page - 1) / page ? table[static_cast<size_t>(src[i]) * W + w] : -1;
+    const int old = table[static_cast<size_t>(dst[i]) * W + w], take = w < pages_of(len, page) ? table[static_cast<size_t>(src[i]) * W + w] : -1;
     if (old != take) {
       if (old >= 0 && old < N) atomicAdd(refs + old, -1);
       if (take >= 0 && take < N) atomicAdd(refs + take, 1);
@@ -127,7 +129,7 @@ __global__ void trim_kernel(int* __restrict__ table, int* __restrict__ lens, int
   if (r < 0 || r >= R) return;
   const int want = to ? to[blockIdx.x] : 0;
   if (want < 0) return;   // this row stays as it is
-  const int len = min(max(0, lens[r]), want), keep = (len + page - 1) / page;
+  const int len = min(max(0, lens[r]), want), keep = min(W, pages_of(len, page));
   for (int w = keep + threadIdx.x; w < W; w += blockDim.x) {
     // (exchanged, so that a row named twice lets go of its pages once)
     const int old = atomicExch(table + static_cast<size_t>(r) * W + w, -1);
@@ -197,7 +199,7 @@ __global__ void __launch_bounds__(kPlanThreads) reserve_plan_kernel(const Reserv
     const long long need = c > 0 ? (static_cast<long long>(len) + c + p.page - 1) / p.page : 0;
     if (need > p.W) atomicExch(&s_too_long, 1);
     plan.need = static_cast<int>(min(need, static_cast<long long>(p.W)));
-    plan.held = min(plan.need, (len + p.page - 1) / p.page);
+    plan.held = min(plan.need, pages_of(len, p.page));
     while (plan.held < plan.need && entry(r, plan.held) >= 0) ++plan.held;   // room from an earlier call
     plan.first = sum;
     sum += (plan.copy >= 0) + plan.need - plan.held;
