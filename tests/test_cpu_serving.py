@@ -66,6 +66,7 @@ def test_shared_prefix_attention_refuses():
     _refused(ValueError, call, scale=float("nan"))
     _refused(ValueError, call, shared=-1)
     _refused(ValueError, call, shared=49)                                  # the table has three pages
+    _refused(ValueError, call, shared=(1 << 30) + 1)                       # lengths and ranges of keys stay in 32 bits
     _refused(ValueError, call, q=ok["q"][:, :3])                           # three query heads for two of the cache
     _refused(ValueError, call, q=ok["q"][..., :32])
     _refused(ValueError, call, q=ok["q"].transpose(0, 1))

@@ -64,6 +64,14 @@ def test_shared_prefix_attention_tiles(B, T, Hq, Hkv, D, page, shared):
     _attention_case(prefix_batch(B, T, Hq, Hkv, D, page, shared, 20, seed=B, device="cuda"), variant="tc")
 
 
+@pytest.mark.parametrize("variant", ["warp", "tc"])
+def test_lengths_below_zero_hold_nothing(variant):
+    c = prefix_batch(24, 3, 8, 2, 64, 64, 200, 40, device="cuda")
+    c["kv_lens"][3:6] = torch.tensor([-1, -2**31, -2**31 + 1], device="cuda", dtype=torch.int32)
+    out = _attention_case(c, variant=variant)
+    assert bool((out[9:18] == 0).all())
+
+
 @pytest.mark.parametrize("B,Hq,Hkv,page,shared,own", [
     (80, 8, 2, 16, 1000, 5000),     # thousands of own keys for one CTA
     (80, 2, 2, 48, 999, 4700),

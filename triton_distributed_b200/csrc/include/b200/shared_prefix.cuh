@@ -25,6 +25,9 @@ struct SharedPrefixParams {
   float scale_log2e;        // softmax scale * log2(e)
 };
 
+constexpr int kPrefixMostKeys = 1 << 30;   // per sequence: sums of a length and a range of keys stay in 32 bits
+__device__ __forceinline__ int prefix_len(const SharedPrefixParams& p, int b) { return min(max(p.kv_lens[b], 0), kPrefixMostKeys); }
+
 bool shared_prefix_tc_takes(const SharedPrefixParams& p, int D);
 int shared_prefix_tc_launch(const SharedPrefixParams& p, int D, int dtype, cudaStream_t s);
 

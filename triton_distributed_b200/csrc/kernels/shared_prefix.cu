@@ -382,7 +382,7 @@ __global__ void __launch_bounds__(kSpanThreads) shared_prefix_span_kernel(const 
         const int g = group * NBP * 8 + r;
         if (g >= p.B * p.T * G) break;
         const int token = g / G;
-        if (p.kv_lens[token / p.T] - p.T + 1 < p.shared) p.lse_part[(static_cast<size_t>(token) * p.Hq + kvh * G + g % G) * p.S + split] = -INFINITY;
+        if (prefix_len(p, token / p.T) - p.T + 1 < p.shared) p.lse_part[(static_cast<size_t>(token) * p.Hq + kvh * G + g % G) * p.S + split] = -INFINITY;
       }
       return;
     }
@@ -396,14 +396,14 @@ __global__ void __launch_bounds__(kSpanThreads) shared_prefix_span_kernel(const 
   const int kvh = at % p.Hkv, b = at / p.Hkv;
   span_fetch_queries<D, NBO>(p, smem, kvh, b * p.T, group * NBO * 8, min(NBO * 8, rows - group * NBO * 8));
   const int* table = p.block_table + static_cast<size_t>(b) * p.bt_stride;
-  const int kv_len = p.kv_lens[b];
+  const int len = prefix_len(p, b);
   // The first pages as they are for a sequence that reaches beyond the shared keys: read together with its length, not after it. (With a window of 32
   // page numbers a warp instead of one ahead, and the merge's outputs fetched before its weights: 2 sequences of 32 / 8 heads, 1000 + 64 keys 8.8 ->
   // 6.9 us; 16 of 64 / 8 heads, 2048 + 512 17.0 -> 14.6; 48 x 3 tokens of 14 / 2 heads of 64, 16384 + 700 33.7 -> 29.0.)
   const bool known = p.own_splits == 1 && p.page % kSpanSlice == 0;
   const int ahead_base = known ? p.shared & ~(kSpanSlice - 1) : -1;
   const int ahead = known ? span_slice_at(p, table, p.width, static_cast<unsigned>(ahead_base) + ((threadIdx.x >> 5) + 4 * (threadIdx.x & 31)) * kSpanSlice) : 0;
-  const int len = max(0, kv_len), start = len - p.T + 1 >= p.shared ? p.shared : 0;
+  const int start = len - p.T + 1 >= p.shared ? p.shared : 0;
   int chunk = (len - start + p.own_splits - 1) / p.own_splits;
   chunk = (chunk + 4 * kSpanSlice - 1) / (4 * kSpanSlice) * (4 * kSpanSlice);
   const int t0 = start + split * chunk, t1 = min(len, t0 + chunk);
@@ -512,7 +512,7 @@ B200_API int b200_shared_prefix_attention(const void* q, long long ldq, const vo
   B200_REQUIRE(dtype == kBF16 || dtype == kF16, "shared-prefix attention supports bf16/f16");
   B200_REQUIRE(D == 64 || D == 128, "shared-prefix attention supports head sizes 64 and 128, got %d", D);
   B200_REQUIRE(Hkv > 0 && Hq > 0 && Hq % Hkv == 0, "Hq (%d) must be a multiple of Hkv (%d)", Hq, Hkv);
-  B200_REQUIRE(B >= 0 && T >= 1 && page >= 1 && num_blocks >= 1 && width >= 0 && shared >= 0 && ldq % 8 == 0, "shared-prefix attention: bad sizes");
+  B200_REQUIRE(B >= 0 && T >= 1 && page >= 1 && num_blocks >= 1 && width >= 0 && shared >= 0 && shared <= kPrefixMostKeys && ldq % 8 == 0, "shared-prefix attention: bad sizes");
   B200_REQUIRE(scale > 0.f, "the score scale must be positive");
   B200_REQUIRE(own_splits >= 1 && (shared == 0 ? prefix_splits == 0 : prefix_splits >= 1), "shared-prefix attention: bad split counts");
   if (B == 0) return kOk;

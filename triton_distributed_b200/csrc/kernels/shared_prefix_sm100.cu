@@ -273,7 +273,7 @@ shared_prefix_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
     const int steps = steps_of(t);
     const int token = token0_of(t) + row / G;
     const bool mine = row < tile_rows && token < all_tokens;
-    const bool valid = mine && n_steps > 0 && p.kv_lens[token / p.T] - p.T + 1 >= p.shared;   // (else the sequence ends inside the shared keys)
+    const bool valid = mine && n_steps > 0 && prefix_len(p, token / p.T) - p.T + 1 >= p.shared;   // (else the sequence ends inside the shared keys)
     float ref = -INFINITY, sum = 0.f;   // the row's reference (of scaled scores) and the sum of 2^(score - reference)
     bool ok = true;
     for (int j = 0; j < steps; ++j) {

@@ -1104,7 +1104,7 @@ def shared_prefix_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: tor
     blocks = -(-shared // page)
     if not scale > 0:
         raise ValueError("shared_prefix_attention: the score scale must be positive")
-    if shared < 0 or (shared > 0 and prefix_table is None and (width < blocks or B == 0)):
+    if not 0 <= shared <= 1 << 30 or (shared > 0 and prefix_table is None and (width < blocks or B == 0)):
         raise ValueError(f"shared_prefix_attention: {shared} shared keys do not fit the block table")
     if prefix_table is not None and (prefix_table.dim() != 1 or prefix_table.shape[0] < blocks or not prefix_table.is_contiguous()):
         raise ValueError("shared_prefix_attention: the prefix table holds the pages of the shared keys")
