@@ -9,8 +9,9 @@
 //
 // This file holds the kernel on warp-level products (m16n8k16) with the keys on the wide side: S^T [16 keys, 8 rows] = K Q^T and O^T [D, 8 rows]
 // += V^T P^T, for 8, 16 or 32 rows that share a KV head per CTA. Each of the four warps streams its own slices of 16 keys through a
-// private ring of three (cp.async, no barrier of the CTA in the loop), its running maximum, sum and output in registers; a slice without a
-// new maximum of any row rescales nothing (one vote). It takes the own keys of every sequence and, while the rows per KV head are few,
+// private ring of three (cp.async, no barrier of the CTA in the loop), its reference, sum and output in registers; the reference is the
+// maximum when it was last raised, and a slice in which no row's score lies more than 8 above it rescales nothing (one vote; 64 / 8 heads, 32768 + 1024
+// keys: 93.7 -> 92.7 us). It takes the own keys of every sequence and, while the rows per KV head are few,
 // the shared keys; both in one launch, the shared ones first because their CTAs run longest. What bounds it is the read of the keys, and in short
 // sequences the latency of starting and merging. The first form, with the rows on the 16 rows of the product, took 1136 instructions a
 // slice and fetched them from beyond the instruction cache (86 us for the own keys of 64 sequences of 544 keys, 8 KV heads).
@@ -32,6 +33,7 @@ namespace b200 {
 constexpr int kSpanThreads = 128;
 constexpr int kSpanSlice = 16;   // keys per slice of a warp
 constexpr int kSpanRing = 3;     // slices in flight per warp
+constexpr float kSpanRaise = 8.f;   // a score (as a power of two) so far above its row's reference raises it; weights are up to 2^8
 
 constexpr int kSpanMostRows = 32;   // per CTA
 template <int D>
@@ -239,7 +241,7 @@ __device__ __forceinline__ void span_body(const SharedPrefixParams& p, uint8_t* 
         }
       }
 #pragma unroll
-      for (int h = 0; h < 2; ++h) raise |= fmaxf(v[nb][h], v[nb][h + 2]) > m_run[nb][h];
+      for (int h = 0; h < 2; ++h) raise |= fmaxf(v[nb][h], v[nb][h + 2]) > m_run[nb][h] + kSpanRaise;
     }
     if (__any_sync(0xffffffffu, raise)) {
 #pragma unroll
@@ -260,7 +262,7 @@ __device__ __forceinline__ void span_body(const SharedPrefixParams& p, uint8_t* 
           }
         }
     }
-    // the weights are rounded to the type of the values: the product's operand has it (a row's largest is one, exactly)
+    // the weights are rounded to the type of the values: the product's operand has it (each relative to itself, also those above one)
     uint32_t pb[NB][2];
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb) {
