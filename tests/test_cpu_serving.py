@@ -153,3 +153,32 @@ def test_prefix_splits_cover_the_keys(B, T, heads, kv, shared, own, page, varian
     tc, prefix, mine = ops.choose_prefix_splits(B, T, heads, kv, shared, own, page, variant=variant)
     assert tc == (variant == "tc") or variant is None
     assert (prefix == 0) == (shared == 0) and 1 <= mine <= 64 and prefix <= 64
+
+
+def _pool_of_two(free=0):
+    """Row 0 holds 28 tokens, row 1 is a fork of it that was cut back to 20: both hold the page of tokens 16 ... 31."""
+    pool = PagePool(1, 2 + free, 2, 64, 1, 8, torch.float32, page_size=16, device="cpu")
+    pool.block_table[:, :2] = torch.tensor([0, 1])
+    pool.kv_lens[:] = torch.tensor([28, 20])
+    pool.refs[:2] = 2
+    return pool
+
+
+@pytest.mark.parametrize("counts,free", [([2, 2], 0), ([0, 0], 4), ([2, 0], 0)])
+def test_pool_slots_are_in_no_page_that_others_hold(counts, free):
+    """A row that got no copy of a page that others hold (too few pages were free, or it asked for none) writes to the spare page."""
+    pool = _pool_of_two(free)
+    status, table, refs, _ = ref.reserve_pages_ref(pool.block_table, pool.kv_lens, pool.refs, torch.tensor(counts), 16)
+    assert status == (1 if any(counts) else 0)
+    pool.block_table.copy_(table), pool.refs.copy_(refs)
+    spare = (2 + free) * 16
+    assert pool.slots(2).tolist() == [spare + 12, spare + 13, spare + 4, spare + 5]
+
+
+def test_pool_slots_of_a_row_that_pauses():
+    """Row 0 goes on in a copy and row 1 pauses: the page is row 1's alone then, and its next slots hold nobody's tokens."""
+    pool = _pool_of_two(3)
+    status, table, refs, copies = ref.reserve_pages_ref(pool.block_table, pool.kv_lens, pool.refs, torch.tensor([2, 0]), 16)
+    pool.block_table.copy_(table), pool.refs.copy_(refs)
+    assert status == 0 and copies == [(1, 2, 12)]
+    assert pool.slots(2).tolist() == [2 * 16 + 12, 2 * 16 + 13, 16 + 4, 16 + 5]

@@ -616,3 +616,33 @@ def test_empty_calls():
     c = draft_batch(0, 2, 5, sampled=False, device="cuda")
     accepted, tokens = ops.verify_drafts(**c)
     assert accepted.shape == (0,) and tokens.shape == (0, 3)
+
+
+def test_rows_without_a_copy_write_nobodys_tokens():
+    """Rows of different length that hold one page: a step that finds no page for the copies, and a step in which both pause, leave the tokens of all rows
+    as they were, captured and replayed too."""
+    from triton_distributed_b200.models import PagePool
+    pool = PagePool(1, 2, 2, 64, 1, 8, torch.float32, page_size=16)
+    n = torch.tensor([28, 0], dtype=torch.int32, device="cuda")
+    pool.reserve(n)
+    _write(pool, 0, pool.slots(28)[:28], *torch.randn(2, 28, 1, 8, device="cuda"))
+    pool.advance(n)
+    pool.fork([0], [1])
+    pool.trim(torch.tensor([28, 20], dtype=torch.int32, device="cuda"))
+    assert pool.refs.tolist() == [2, 2]
+    tokens, state = pool.k_cache[:, :2].clone(), [t.clone() for t in (pool.block_table, pool.refs)]
+
+    def step(count):
+        pool.reserve(count, check=False)
+        _write(pool, 0, pool.slots(2), torch.full((4, 1, 8), 7.0, device="cuda"), torch.full((4, 1, 8), 7.0, device="cuda"))
+
+    counts = [torch.tensor(c, dtype=torch.int32, device="cuda") for c in ([2, 2], [2, 0], [0, 0])]
+    for count in counts:
+        step(count)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        step(counts[0])
+    g.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(pool.k_cache[:, :2], tokens)
+    _same((pool.block_table, pool.refs), state)

@@ -156,7 +156,7 @@ class PagePool:
     ``refs`` int32 [num_blocks] (how many rows hold a page) live on the device and are changed in place by kernels, so that a step can be
     captured. A step of S tokens: ``reserve(S)``, keys and values to ``slots(S)``, ``advance(S)``, attention over ``layer(i)``, ``kv_lens`` and
     ``block_table`` (``ops.decode_attention``, ``ops.shared_prefix_attention``); drafts that were refused go with ``trim``. The caches have one page
-    more than ``refs`` counts: rows without room write there."""
+    more than ``refs`` counts: rows without room of their own write there."""
 
     def __init__(self, num_layers: int, num_blocks: int, batch_size: int, max_length: int, kv_heads: int, head_dim: int = 128, dtype=torch.bfloat16,
                  page_size: int = 64, device="cuda") -> None:
@@ -192,11 +192,14 @@ class PagePool:
             raise RuntimeError("PagePool: too few free pages" if code == 1 else "PagePool: a row would exceed max_length")
 
     def slots(self, count: int) -> torch.Tensor:
-        """Flat slot (page * page_size + offset) of the next `count` tokens of every row -> int64 [batch * count]; the spare page for rows without room."""
+        """Flat slot (page * page_size + offset) of the next `count` tokens of every row -> int64 [batch * count]. What has no room is sent to the spare
+        page: positions without a page, and those in a page that other rows hold too (their tokens may lie there: a row that paused, or whose
+        ``reserve`` failed, has got no copy of it). So forks come before the ``reserve`` of a step."""
         pos = self.kv_lens[:, None].to(torch.int64) + torch.arange(count, device=self.kv_lens.device)[None, :]
         at = pos // self.page_size
         blk = self.block_table.gather(1, at.clamp_max(self.block_table.shape[1] - 1)).to(torch.int64)
-        blk = torch.where((blk >= 0) & (at < self.block_table.shape[1]), blk, self.num_blocks)
+        alone = self.refs[blk.clamp(0, self.num_blocks - 1)] <= 1
+        blk = torch.where((blk >= 0) & (at < self.block_table.shape[1]) & alone, blk, self.num_blocks)
         return (blk * self.page_size + pos % self.page_size).reshape(-1)
 
     def advance(self, count) -> None:
