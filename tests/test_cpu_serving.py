@@ -182,3 +182,14 @@ def test_pool_slots_of_a_row_that_pauses():
     pool.block_table.copy_(table), pool.refs.copy_(refs)
     assert status == 0 and copies == [(1, 2, 12)]
     assert pool.slots(2).tolist() == [2 * 16 + 12, 2 * 16 + 13, 16 + 4, 16 + 5]
+
+
+def test_pool_check_looks_once():
+    pool = _pool_of_two()
+    for code in (1, 2):
+        pool.status.fill_(code)
+        with pytest.raises(RuntimeError):
+            pool.check()
+        pool.check()
+    table, lens, refs = page_state(6, 4, 30, 8)
+    _refused(ValueError, ops.reserve_pages, table, lens, refs, 1, [torch.zeros(30, 8, 4)], keep=True)   # there is no status to keep

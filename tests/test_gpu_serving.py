@@ -646,3 +646,28 @@ def test_rows_without_a_copy_write_nobodys_tokens():
     torch.cuda.synchronize()
     assert torch.equal(pool.k_cache[:, :2], tokens)
     _same((pool.block_table, pool.refs), state)
+
+
+def test_a_reserve_that_failed_is_remembered():
+    """The outcome of an unchecked reserve (of a captured step) is there after later ones that found room, and is gone once it has been looked at."""
+    from triton_distributed_b200 import ops
+    from triton_distributed_b200.models import PagePool
+    pool = PagePool(1, 3, 2, 64, 1, 8, torch.float32, page_size=16)
+    g = torch.cuda.CUDAGraph()
+    count = torch.tensor([16, 48], dtype=torch.int32, device="cuda")
+    pool.reserve(torch.zeros_like(count))
+    with torch.cuda.graph(g):
+        pool.reserve(count, check=False)
+    for counts, code, after in (([16, 48], 1, 1), ([16, 0], 0, 1), ([16, 64], 1, 1), ([65, 0], 2, 2), ([16, 0], 0, 2)):
+        count.copy_(torch.tensor(counts, dtype=torch.int32))
+        g.replay()
+        assert int(pool.status) == after
+        alone = ops.reserve_pages(pool.block_table.clone(), pool.kv_lens, pool.refs.clone(), count, (pool.k_cache.clone(), pool.v_cache.clone()), dim=1)
+        assert int(alone) == code
+    with pytest.raises(RuntimeError, match="max_length"):
+        pool.check()
+    pool.check()
+    pool.reserve(count)
+    with pytest.raises(RuntimeError, match="free pages"):
+        pool.reserve(torch.tensor([16, 64], dtype=torch.int32, device="cuda"))
+    pool.reserve(count)

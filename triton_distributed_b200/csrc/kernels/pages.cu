@@ -161,6 +161,7 @@ struct ReserveParams {
   int4* moves;         // [R]
   int* n_moves;
   int* status;
+  int keep;            // whether *status is raised to this outcome, but never lowered
 };
 __global__ void __launch_bounds__(kPlanThreads) reserve_plan_kernel(const ReserveParams p) {
   __shared__ int warp_sums[32];
@@ -262,7 +263,8 @@ __global__ void __launch_bounds__(kPlanThreads) reserve_plan_kernel(const Reserv
   __syncthreads();
   if (tid == 0) {
     *p.n_moves = s_moves;
-    *p.status = s_too_long ? 2 : total > found ? 1 : 0;
+    const int outcome = s_too_long ? 2 : total > found ? 1 : 0;
+    *p.status = p.keep ? max(*p.status, outcome) : outcome;
   }
 }
 
@@ -464,9 +466,10 @@ B200_API int b200_trim_pages(int* table, int* lens, int* refs, const int* rows, 
 // int32 words of scratch that b200_reserve_pages and b200_compact_pages need (16-byte aligned).
 B200_API long long b200_pages_scratch(int R, int N) { return 8LL * R + 8LL * N + 16; }
 
-// Room for counts[r] (null: count) more tokens in every row, see ReserveParams; the copies are made in `tensors`.
+// Room for counts[r] (null: count) more tokens in every row, see ReserveParams; the copies are made in `tensors`. keep: *status becomes the larger of
+// what it was and this call's outcome.
 B200_API int b200_reserve_pages(int* table, const int* lens, int* refs, const int* counts, int count, int R, int W, int N, int page, const void* tensors,
-                                int n_tensors, int* scratch, int* status, void* stream) {
+                                int n_tensors, int* scratch, int* status, int keep, void* stream) {
   B200_REQUIRE(R >= 1 && W >= 1 && N >= 1 && page >= 1 && count >= 0 && n_tensors >= 0, "reserve_pages: bad sizes");
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   ReserveParams p;
@@ -477,7 +480,7 @@ B200_API int b200_reserve_pages(int* table, const int* lens, int* refs, const in
   p.lowest = p.asks + N;
   p.fresh = p.lowest + N;
   p.n_moves = p.fresh + N;
-  p.status = status;
+  p.status = status; p.keep = keep;
   B200_CHECK_CUDA(launch_pdl(reserve_plan_kernel, 1, kPlanThreads, 0, s, p));
   if (n_tensors == 0) return kOk;
   MoveParams m;

@@ -180,15 +180,16 @@ class PagePool:
 
     def reserve(self, count, check: bool = True) -> None:
         """Room for `count` more tokens (a number, or int32 [batch]) in every row (``ops.reserve_pages``). ``check``: wait for the outcome and
-        raise where there are too few pages; without it (inside a capture) ``status`` tells."""
-        ops.reserve_pages(self.block_table, self.kv_lens, self.refs, count, (self.k_cache, self.v_cache), dim=1, status=self.status)
+        raise where there are too few pages; without it (inside a capture) ``status`` keeps the worst outcome until the next ``check``."""
+        ops.reserve_pages(self.block_table, self.kv_lens, self.refs, count, (self.k_cache, self.v_cache), dim=1, status=self.status, keep=True)
         if check:
             self.check()
 
     def check(self) -> None:
-        """Raise if the last ``reserve`` found too few pages, or a row that would outgrow its table (nothing has been changed then)."""
+        """Raise if a ``reserve`` since the last check found too few pages, or a row that would outgrow its table (it has changed nothing then)."""
         code = int(self.status.item())
         if code:
+            self.status.zero_()
             raise RuntimeError("PagePool: too few free pages" if code == 1 else "PagePool: a row would exceed max_length")
 
     def slots(self, count: int) -> torch.Tensor:

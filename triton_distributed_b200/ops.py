@@ -995,7 +995,7 @@ _SERVING_ARGS = {
     "b200_verify_drafts": (_P, _P, _L, _L, _P, _L, _L, _P, _P, _I, _I, _I, _P, _P, _I, _P),
     "b200_fork_pages": (_P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _P, _P),
     "b200_trim_pages": (_P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _P),
-    "b200_reserve_pages": (_P, _P, _P, _P, _I, _I, _I, _I, _I, _P, _I, _P, _P, _P),
+    "b200_reserve_pages": (_P, _P, _P, _P, _I, _I, _I, _I, _I, _P, _I, _P, _P, _I, _P),
     "b200_compact_pages": (_P, _P, _P, _P, _I, _I, _I, _I, _P, _I, _P, _P),
     "b200_copy_pages": (_P, _I, _P, _I, _I, _P),
 }
@@ -1244,14 +1244,15 @@ def trim_pages(block_table: torch.Tensor, kv_lens: torch.Tensor, refs: torch.Ten
 
 
 def reserve_pages(block_table: torch.Tensor, kv_lens: torch.Tensor, refs: torch.Tensor, count, caches, dim: int = 0,
-                  status: torch.Tensor | None = None) -> torch.Tensor:
+                  status: torch.Tensor | None = None, keep: bool = False) -> torch.Tensor:
     """Room for ``count`` more tokens (a number, or int32 [rows]; rows with none are left alone) in every row, in place: the entries up to
     ``ceil((kv_lens + count) / page)`` get free pages (in ascending order, row by row), and a row whose next token falls into a page that others hold
     gets a copy of it (where all its holders ask, the first row keeps it). ``caches``: the tensors that the pages are in, ``[pages, tokens, ...]`` or
     with ``dim=1`` ``[layers, pages, tokens, ...]``. Lengths stay as they are.
 
     Returns ``status`` (int32 [1], on the device): 0, or 1 where too few pages are free and 2 where a row would outgrow the table; then nothing has
-    been changed."""
+    been changed. ``keep``: the given status is raised to this outcome but never lowered, so that a failure among several calls (of a captured step that is
+    replayed) is still there when the host looks."""
     caches, tensors, page = _page_tensors("reserve_pages", caches, dim, refs.numel())
     if not caches:
         raise ValueError("reserve_pages: the caches that hold the pages are needed")
@@ -1267,12 +1268,14 @@ def reserve_pages(block_table: torch.Tensor, kv_lens: torch.Tensor, refs: torch.
             raise ValueError("reserve_pages: the count of tokens is not negative")
     if status is not None and (status.dtype != torch.int32 or status.numel() != 1):
         raise ValueError("reserve_pages: the status is one int32")
+    if keep and status is None:
+        raise ValueError("reserve_pages: what is kept is the status that the caller gives")
     device = _check_device("reserve_pages", block_table, kv_lens, refs, counts, status, *caches)
     if status is None:
         status = refs.new_empty(1)
     scratch = refs.new_empty(8 * (R + N) + 16)   # b200_pages_scratch
     _launch("b200_reserve_pages", 2, device, block_table.data_ptr(), kv_lens.data_ptr(), refs.data_ptr(), _dptr(counts), count, R, W, N, page, tensors, len(caches),
-            scratch.data_ptr(), status.data_ptr())
+            scratch.data_ptr(), status.data_ptr(), int(keep))
     return status
 
 
