@@ -193,3 +193,32 @@ def test_pool_check_looks_once():
         pool.check()
     table, lens, refs = page_state(6, 4, 30, 8)
     _refused(ValueError, ops.reserve_pages, table, lens, refs, 1, [torch.zeros(30, 8, 4)], keep=True)   # there is no status to keep
+
+
+@pytest.mark.parametrize("advanced", [16, 9, 33])
+@pytest.mark.parametrize("held", [0, 1])
+def test_reserve_reference_leaves_no_gap(held, advanced):
+    """A row whose length went on after a reserve that found no room is refused until it is cut back to what it holds."""
+    table, refs = torch.full((2, 5), -1, dtype=torch.int32), torch.zeros(4, dtype=torch.int32)
+    table[0, :held] = torch.arange(held, dtype=torch.int32)
+    table[1, :4 - held] = torch.arange(held, 4, dtype=torch.int32)
+    refs[:] = 1
+    lens = torch.tensor([16 * held, 64 - 16 * held], dtype=torch.int32)
+    asks = torch.tensor([advanced, 0], dtype=torch.int32)
+    status, table, refs, _ = ref.reserve_pages_ref(table, lens, refs, asks, 16)
+    assert status == 1
+    table, lens, refs = ref.trim_pages_ref(table, lens + asks, refs, 16, None, [1])       # advanced unseen; the other row ends
+    before = table.clone(), refs.clone()
+    status, table, refs, copies = ref.reserve_pages_ref(table, lens, refs, torch.tensor([1, 1]), 16)
+    assert status == 3 and not copies and torch.equal(table, before[0]) and torch.equal(refs, before[1])
+    assert ref.reserve_pages_ref(table, lens, refs, torch.tensor([0, 1]), 16)[0] == 0     # rows that do not ask are left alone
+    table, lens, refs = ref.trim_pages_ref(table, lens, refs, 16, torch.tensor([16 * held]), [0])
+    status, table, refs, _ = ref.reserve_pages_ref(table, lens, refs, torch.tensor([1, 1]), 16)
+    assert status == 0 and torch.equal(counts_of(table, 4), refs)
+
+
+def test_pool_check_names_the_gap():
+    pool = _pool_of_two()
+    pool.status.fill_(3)
+    with pytest.raises(RuntimeError, match="last token"):
+        pool.check()

@@ -671,3 +671,29 @@ def test_a_reserve_that_failed_is_remembered():
     with pytest.raises(RuntimeError, match="free pages"):
         pool.reserve(torch.tensor([16, 64], dtype=torch.int32, device="cuda"))
     pool.reserve(count)
+
+
+@pytest.mark.parametrize("advanced", [16, 9, 33])
+@pytest.mark.parametrize("held", [0, 1])
+def test_rows_that_went_on_without_room(held, advanced):
+    """A row whose length was raised after a reserve that found no room gets no pages behind the gap; cut back to what it holds it goes on."""
+    from triton_distributed_b200 import ops
+    from triton_distributed_b200.models import PagePool
+    pool = PagePool(1, 4, 2, 80, 1, 8, torch.float32, page_size=16)
+    first = torch.tensor([16 * held, 64 - 16 * held], dtype=torch.int32, device="cuda")
+    pool.reserve(first), pool.advance(first)
+    asks = torch.tensor([advanced, 0], dtype=torch.int32, device="cuda")
+    pool.reserve(asks, check=False)
+    pool.advance(asks)
+    pool.free([1])
+    with pytest.raises(RuntimeError, match="free pages"):
+        pool.check()
+    state = [t.clone() for t in (pool.block_table, pool.kv_lens, pool.refs)]
+    with pytest.raises(RuntimeError, match="last token"):
+        pool.reserve(1)
+    _same((pool.block_table, pool.kv_lens, pool.refs), state)
+    assert int(ops.reserve_pages(*state, 80, (pool.k_cache, pool.v_cache), dim=1)) == 2      # a row of the table is too short in the first place
+    pool.reserve(torch.tensor([0, 1], dtype=torch.int32, device="cuda"))
+    pool.trim(torch.tensor([16 * held], dtype=torch.int32, device="cuda"), [0])
+    pool.reserve(1)
+    assert torch.equal(counts_of(pool.block_table.cpu(), 4), pool.refs.cpu())

@@ -142,7 +142,8 @@ __global__ void trim_kernel(int* __restrict__ table, int* __restrict__ lens, int
 // ---- room for more tokens --------------------------------------------------------------------
 // One CTA plans: which rows write into a page that others hold (they get a copy; if all its holders write, the first row keeps the page), how
 // many fresh pages each row needs, and which free pages they are. moves[k] = {from, to, tokens, 0} for the copies, *n_moves their number.
-// If there are too few pages, or a row becomes too long for the table, nothing is changed: *status says so and *n_moves is zero.
+// If there are too few pages (1), a row becomes too long for the table (2) or has no page for its last token (3: its length went on after a call that
+// found no room, and pages behind the gap would be attended as if the gap held keys), nothing is changed: *status says so and *n_moves is zero.
 struct RowPlan {
   int copy;         // the page that is copied, or -1
   int held, need;   // entries [held, need) are given fresh pages
@@ -165,11 +166,11 @@ struct ReserveParams {
 };
 __global__ void __launch_bounds__(kPlanThreads) reserve_plan_kernel(const ReserveParams p) {
   __shared__ int warp_sums[32];
-  __shared__ int s_too_long, s_moves, s_n_long, s_long[kLongRows];
+  __shared__ int s_too_long, s_gap, s_moves, s_n_long, s_long[kLongRows];
   griddep_wait();
   griddep_launch_dependents();
   const int tid = threadIdx.x;
-  if (tid == 0) { s_too_long = 0; s_moves = 0; s_n_long = 0; }
+  if (tid == 0) { s_too_long = 0; s_gap = 0; s_moves = 0; s_n_long = 0; }
   const int each = (p.R + kPlanThreads - 1) / kPlanThreads;   // thread t plans rows [t * each, (t + 1) * each)
   const int r0 = min(p.R, tid * each), r1 = min(p.R, r0 + each);
   auto entry = [&](int r, int w) -> int& { return p.table[static_cast<size_t>(r) * p.W + w]; };
@@ -199,6 +200,7 @@ __global__ void __launch_bounds__(kPlanThreads) reserve_plan_kernel(const Reserv
     if (plan.copy >= 0 && __ldcg(p.asks + plan.copy) == p.refs[plan.copy] && __ldcg(p.lowest + plan.copy) == r) plan.copy = -1;
     const long long need = c > 0 ? (static_cast<long long>(len) + c + p.page - 1) / p.page : 0;
     if (need > p.W) atomicExch(&s_too_long, 1);
+    else if (need > 0 && len > 0 && entry(r, pages_of(len, p.page) - 1) < 0) atomicExch(&s_gap, 1);
     plan.need = static_cast<int>(min(need, static_cast<long long>(p.W)));
     plan.held = min(plan.need, pages_of(len, p.page));
     while (plan.held < plan.need && entry(r, plan.held) >= 0) ++plan.held;   // room from an earlier call
@@ -223,7 +225,7 @@ __global__ void __launch_bounds__(kPlanThreads) reserve_plan_kernel(const Reserv
     if (c.w <= 0 && k < total) p.fresh[k] = i + 3;
     found += in_tile;
   }
-  const bool fits = s_too_long == 0 && total <= found;
+  const bool fits = s_too_long == 0 && s_gap == 0 && total <= found;
   __syncthreads();
   if (fits) {
     for (int r = r0; r < r1; ++r) {
@@ -263,7 +265,7 @@ __global__ void __launch_bounds__(kPlanThreads) reserve_plan_kernel(const Reserv
   __syncthreads();
   if (tid == 0) {
     *p.n_moves = s_moves;
-    const int outcome = s_too_long ? 2 : total > found ? 1 : 0;
+    const int outcome = s_too_long ? 2 : s_gap ? 3 : total > found ? 1 : 0;
     *p.status = p.keep ? max(*p.status, outcome) : outcome;
   }
 }

@@ -186,11 +186,12 @@ class PagePool:
             self.check()
 
     def check(self) -> None:
-        """Raise if a ``reserve`` since the last check found too few pages, or a row that would outgrow its table (it has changed nothing then)."""
+        """Raise if a ``reserve`` since the last check found too few pages, a row that would outgrow its table or one without a page for its last token (it
+        has changed nothing then). Rows that were advanced all the same count tokens that no page holds: ``trim`` or ``free`` them."""
         code = int(self.status.item())
         if code:
             self.status.zero_()
-            raise RuntimeError("PagePool: too few free pages" if code == 1 else "PagePool: a row would exceed max_length")
+            raise RuntimeError("PagePool: " + {1: "too few free pages", 2: "a row would exceed max_length"}.get(code, "a row has no page for its last token"))
 
     def slots(self, count: int) -> torch.Tensor:
         """Flat slot (page * page_size + offset) of the next `count` tokens of every row -> int64 [batch * count]. What has no room is sent to the spare

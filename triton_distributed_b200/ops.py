@@ -1250,8 +1250,8 @@ def reserve_pages(block_table: torch.Tensor, kv_lens: torch.Tensor, refs: torch.
     gets a copy of it (where all its holders ask, the first row keeps it). ``caches``: the tensors that the pages are in, ``[pages, tokens, ...]`` or
     with ``dim=1`` ``[layers, pages, tokens, ...]``. Lengths stay as they are.
 
-    Returns ``status`` (int32 [1], on the device): 0, or 1 where too few pages are free and 2 where a row would outgrow the table; then nothing has
-    been changed. ``keep``: the given status is raised to this outcome but never lowered, so that a failure among several calls (of a captured step that is
+    Returns ``status`` (int32 [1], on the device): 0, or 1 where too few pages are free, 2 where a row would outgrow the table and 3 where a row that asks
+    has no page for its last token (its length was raised although an earlier call had found no room: trim it to what it holds); then nothing has been changed. ``keep``: the given status is raised to this outcome but never lowered, so that a failure among several calls (of a captured step that is
     replayed) is still there when the host looks."""
     caches, tensors, page = _page_tensors("reserve_pages", caches, dim, refs.numel())
     if not caches:

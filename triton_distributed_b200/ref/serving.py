@@ -122,7 +122,7 @@ def reserve_pages_ref(block_table, kv_lens, refs, count, page_size: int):
                 part.setdefault(pg, []).append(r)
     copies_of = {r: pg for pg, rs in part.items() for r in (rs[1:] if len(rs) == int(refs[pg]) else rs)}
     free = [i for i in range(refs.numel()) if int(refs[i]) <= 0]
-    copies, given = [], 0
+    copies, given, gap = [], 0, False
 
     def take():
         nonlocal given
@@ -136,6 +136,7 @@ def reserve_pages_ref(block_table, kv_lens, refs, count, page_size: int):
         need = -(-(n + c) // page_size)
         if need > W:
             return 2, block_table.clone(), refs.clone(), []
+        gap = gap or (n > 0 and int(block_table[r, -(-n // page_size) - 1]) < 0)
         held = -(-n // page_size)
         while held < need and int(table[r, held]) >= 0:
             held += 1
@@ -148,6 +149,8 @@ def reserve_pages_ref(block_table, kv_lens, refs, count, page_size: int):
         for w in range(held, need):
             table[r, w] = take()
             new[table[r, w].long()] = 1
+    if gap:
+        return 3, block_table.clone(), refs.clone(), []
     if given > len(free):
         return 1, block_table.clone(), refs.clone(), []
     return 0, table, new, copies
