@@ -222,3 +222,13 @@ def test_pool_check_names_the_gap():
     pool.status.fill_(3)
     with pytest.raises(RuntimeError, match="last token"):
         pool.check()
+
+
+@pytest.mark.parametrize("heads,tokens", [(128, 131070), (64, 262140), (43, 262140), (1, 16776960)])
+def test_rows_that_no_grid_of_tiles_holds(heads, tokens):
+    """Pairs of tiles of 128 // heads tokens are counted by the second dimension of a grid, 65535 at most: more rows go to the warp kernel."""
+    choice = lambda n, **kw: ops.choose_prefix_splits(1, n, heads, 1, 1024, n, **kw)[0]  # noqa: E731
+    assert choice(tokens) and choice(tokens, variant="tc")
+    assert not choice(tokens + 1) and not choice(tokens + 1, variant="warp")
+    with pytest.raises(ValueError):
+        choice(tokens + 1, variant="tc")

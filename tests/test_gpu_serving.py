@@ -697,3 +697,21 @@ def test_rows_that_went_on_without_room(held, advanced):
     pool.trim(torch.tensor([16 * held], dtype=torch.int32, device="cuda"), [0])
     pool.reserve(1)
     assert torch.equal(counts_of(pool.block_table.cpu(), 4), pool.refs.cpu())
+
+
+def test_more_rows_than_a_grid_of_tiles_holds():
+    """131071 sequences with 128 query heads on one KV head: a tile holds one token, and there are more pairs of tiles than a grid counts."""
+    from triton_distributed_b200 import ops, ref
+    B, D, page = 131071, 64, 64
+    g = torch.Generator(device="cuda").manual_seed(1)
+    k, v = (torch.randn(9, page, 1, D, device="cuda", generator=g).bfloat16() for _ in range(2))
+    table = torch.zeros(B, 2, dtype=torch.int32, device="cuda")
+    table[:, 1] = 1 + torch.arange(B, device="cuda") % 8
+    lens = (65 + torch.arange(B, device="cuda") % 50).int()
+    q = torch.randn(B, 128, D, device="cuda", generator=g, dtype=torch.bfloat16)
+    out, lse = ops.shared_prefix_attention(q, k, v, lens, table, 64, 0.125, return_lse=True)
+    some = torch.tensor([0, 1, 4097, 65534, 65535, 65536, B - 2, B - 1], device="cuda")
+    c = {"q": q[some], "k_cache": k, "v_cache": v, "kv_lens": lens[some], "block_table": table[some], "shared": 64, "scale": 0.125}
+    want, want_lse = ref.shared_prefix_attention_ref(**c)
+    spread, _ = ref.shared_prefix_attention_ref(**{**c, "v_cache": v.abs()})
+    _check_attention(c, out[some], lse[some], want, want_lse, spread)

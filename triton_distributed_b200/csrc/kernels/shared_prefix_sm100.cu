@@ -474,16 +474,21 @@ static int launch_prefix(const CUtensorMap& tq, const CUtensorMap& tk, const CUt
   return kOk;
 }
 
+static int row_tiles(const SharedPrefixParams& p) {
+  const int tokens = kXM / (p.Hq / p.Hkv);   // of a tile
+  return (p.B * p.T + tokens - 1) / tokens;
+}
+
 // Whether the kernel handles a call at all: whole groups of query heads in a tile, pages of whole swizzle atoms (8 keys), slots that a 32-bit
-// coordinate reaches.
+// coordinate reaches, pairs of tiles and KV heads that a grid holds.
 bool shared_prefix_tc_takes(const SharedPrefixParams& p, int D) {
   return p.shared > 0 && p.Hq / p.Hkv <= kXM && (D == 64 || D == 128) && p.page % 8 == 0 &&
-         static_cast<long long>(p.num_blocks) * p.page < 0x7fffff00LL && p.Hkv <= 65535;
+         static_cast<long long>(p.num_blocks) * p.page < 0x7fffff00LL && p.Hkv <= 65535 && row_tiles(p) <= 2 * 65535;
 }
 
 // p.prefix_splits ranges of p.prefix_chunk keys (a multiple of 128).
 int shared_prefix_tc_launch(const SharedPrefixParams& p, int D, int dtype, cudaStream_t s) {
-  const int G = p.Hq / p.Hkv, tile_tokens = kXM / G, tiles = (p.B * p.T + tile_tokens - 1) / tile_tokens;
+  const int G = p.Hq / p.Hkv, tile_tokens = kXM / G, tiles = row_tiles(p);
   const bool two_ranges = tiles == 1;
   const int rows = prefix_copy_rows(p.page);
   const uint64_t slots = static_cast<uint64_t>(p.num_blocks) * p.page;
@@ -493,7 +498,6 @@ int shared_prefix_tc_launch(const SharedPrefixParams& p, int D, int dtype, cudaS
   if (rc == kOk) rc = make_tma_3d(&tv, p.v_cache, dtype, D, p.Hkv, slots, D, static_cast<uint64_t>(p.Hkv) * D, 64, 1, rows, true);
   if (rc != kOk) return rc;
   const dim3 grid(p.prefix_splits, two_ranges ? 1 : (tiles + 1) / 2, p.Hkv);
-  B200_REQUIRE(grid.y <= 65535, "shared-prefix attention: too many rows");
 #define B200_PREFIX(A, TWO) (dtype == kBF16 ? launch_prefix<A, true, TWO>(tq, tk, tv, p, grid, s) : launch_prefix<A, false, TWO>(tq, tk, tv, p, grid, s))
   if (D == 128) return two_ranges ? B200_PREFIX(2, true) : B200_PREFIX(2, false);
   return two_ranges ? B200_PREFIX(1, true) : B200_PREFIX(1, false);

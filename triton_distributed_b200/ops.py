@@ -1035,7 +1035,8 @@ def choose_prefix_splits(batch: int, tokens: int, heads: int, kv_heads: int, sha
     rows = batch * tokens * group
     blocks = lambda n: -(-n // (8 if n <= 8 else 16 if n <= 16 else 32))  # noqa: E731  (CTAs for n rows of the warp kernel)
     own_ctas = batch * kv_heads * blocks(tokens * group)
-    able = shared > 0 and group <= 128 and page % 8 == 0 and slots < 0x7fffff00 and kv_heads <= 65535
+    tiles = -(-batch * tokens // (128 // group)) if group <= 128 else 0
+    able = shared > 0 and 0 < tiles <= 2 * 65535 and page % 8 == 0 and slots < 0x7fffff00 and kv_heads <= 65535
     if variant == "tc" and not able:
         raise ValueError("shared_prefix_attention: these heads or pages are not for the tensor-core kernel")
     tc = able and (rows > 16 if variant is None else variant == "tc")
@@ -1049,7 +1050,6 @@ def choose_prefix_splits(batch: int, tokens: int, heads: int, kv_heads: int, sha
     own_splits = 1
     while own_splits < 64 and own_ctas * own_splits < sm_count // 2 and own > 256 * own_splits:
         own_splits += 1
-    tiles = -(-batch * tokens // (128 // group))
     units, steps, ctas = kv_heads * -(-tiles // 2), -(-shared // 128), own_ctas * own_splits
     step_us, merge_us = 0.95 if tiles == 1 else 1.9, batch * tokens * heads * dim * 8 / 3e6
     own_us = 5 + 0.018 * own / 2 / own_splits
