@@ -232,3 +232,11 @@ def test_rows_that_no_grid_of_tiles_holds(heads, tokens):
     assert not choice(tokens + 1) and not choice(tokens + 1, variant="warp")
     with pytest.raises(ValueError):
         choice(tokens + 1, variant="tc")
+
+
+def test_rows_outside_32_bits_stay_outside():
+    """Row numbers that 32 bits do not hold name no row, not the one with the same low bits."""
+    far = [2**32, 2**32 + 3, -2**32, 2**31, -2**31 - 1, 2**63 - 1, -2**63, -1, 5]
+    for rows in (far, torch.tensor(far)):
+        got = ops._rows("fork_pages", rows, torch.device("cpu"))
+        assert got.dtype == torch.int32 and got[-1] == 5 and bool(((got[:-1] < 0) | (got[:-1] == 2**31 - 1)).all())

@@ -715,3 +715,16 @@ def test_more_rows_than_a_grid_of_tiles_holds():
     want, want_lse = ref.shared_prefix_attention_ref(**c)
     spread, _ = ref.shared_prefix_attention_ref(**{**c, "v_cache": v.abs()})
     _check_attention(c, out[some], lse[some], want, want_lse, spread)
+
+
+def test_rows_that_32_bits_do_not_hold_are_skipped():
+    from triton_distributed_b200 import ops, ref
+    state = page_state(9, 5, 60, 4, 3)
+    got = [t.cuda() for t in state]
+    far = torch.tensor([2**32 + 3, 0, 2**32, -2**32 + 1], device="cuda")
+    ops.fork_pages(*got, far, [1, 2**32 + 2, 4, 5], 4)
+    ops.fork_pages(*got, [2**32] * 300, [7] * 300, 4)
+    ops.trim_pages(*got, 4, None, far[[0, 2, 3]])
+    _same(got, state)
+    ops.trim_pages(*got, 4, None, far)
+    _same(got, ref.trim_pages_ref(*state, 4, None, [0]))

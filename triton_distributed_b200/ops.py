@@ -1202,12 +1202,14 @@ def _check_page_state(name: str, block_table, refs, kv_lens=None, page=1) -> tup
 
 def _rows(name: str, rows, device) -> torch.Tensor:
     if not isinstance(rows, torch.Tensor):
-        rows = torch.as_tensor(rows, device=device)
+        rows = torch.as_tensor(rows)
     if rows.dim() != 1 or (rows.dtype not in (torch.int32, torch.int64) and rows.numel()):
         raise ValueError(f"{name}: rows are a list or a 1-D tensor of whole numbers")
     if rows.dtype == torch.int32 and rows.is_contiguous() and rows.device == device:
         return rows
-    return rows.to(device=device, dtype=torch.int32).contiguous()
+    if rows.dtype == torch.int64:
+        rows = rows.clamp(-1, 2**31 - 1)   # what 32 bits do not hold stays outside the table
+    return rows.to(torch.int32).to(device).contiguous()
 
 
 def fork_pages(block_table: torch.Tensor, kv_lens: torch.Tensor, refs: torch.Tensor, src, dst, page_size: int) -> None:
