@@ -240,3 +240,9 @@ def test_rows_outside_32_bits_stay_outside():
     for rows in (far, torch.tensor(far)):
         got = ops._rows("fork_pages", rows, torch.device("cpu"))
         assert got.dtype == torch.int32 and got[-1] == 5 and bool(((got[:-1] < 0) | (got[:-1] == 2**31 - 1)).all())
+
+
+@pytest.mark.parametrize("R,N", [(1, 1), (9, 60), (1500, 70000), (2**20, 2**27)])
+def test_pages_scratch_holds_both_layouts(R, N):
+    """Room: moves (4 words) and plans (4) of the rows, three lists of pages, a count. Compaction: moves (4 words) and three lists of pages, a count."""
+    assert ops._pages_scratch(R, N) >= max(8 * R + 3 * N + 1, 7 * N + 1)

@@ -465,7 +465,7 @@ B200_API int b200_trim_pages(int* table, int* lens, int* refs, const int* rows, 
   return kOk;
 }
 
-// int32 words of scratch that b200_reserve_pages and b200_compact_pages need (16-byte aligned).
+// int32 words of scratch that b200_reserve_pages (8 R + 3 N + 1) and b200_compact_pages (7 N + 1) need (16-byte aligned).
 B200_API long long b200_pages_scratch(int R, int N) { return 8LL * R + 8LL * N + 16; }
 
 // Room for counts[r] (null: count) more tokens in every row, see ReserveParams; the copies are made in `tensors`. keep: *status becomes the larger of

@@ -1200,6 +1200,14 @@ def _check_page_state(name: str, block_table, refs, kv_lens=None, page=1) -> tup
     return *block_table.shape, refs.shape[0]
 
 
+@functools.lru_cache(maxsize=256)
+def _pages_scratch(rows: int, pages: int) -> int:
+    """int32 words of scratch that reserve_pages and compact_pages need."""
+    fn = _lib.load().b200_pages_scratch
+    fn.argtypes, fn.restype = (_I, _I), _L
+    return fn(rows, pages)
+
+
 def _rows(name: str, rows, device) -> torch.Tensor:
     if not isinstance(rows, torch.Tensor):
         rows = torch.as_tensor(rows)
@@ -1275,7 +1283,7 @@ def reserve_pages(block_table: torch.Tensor, kv_lens: torch.Tensor, refs: torch.
     device = _check_device("reserve_pages", block_table, kv_lens, refs, counts, status, *caches)
     if status is None:
         status = refs.new_empty(1)
-    scratch = refs.new_empty(8 * (R + N) + 16)   # b200_pages_scratch
+    scratch = refs.new_empty(_pages_scratch(R, N))
     _launch("b200_reserve_pages", 2, device, block_table.data_ptr(), kv_lens.data_ptr(), refs.data_ptr(), _dptr(counts), count, R, W, N, page, tensors, len(caches),
             scratch.data_ptr(), status.data_ptr(), int(keep))
     return status
@@ -1292,7 +1300,7 @@ def compact_pages(block_table: torch.Tensor, refs: torch.Tensor, caches, dim: in
     elif out[0].shape != block_table.shape or out[1].shape != refs.shape or any(t.dtype != torch.int32 or not t.is_contiguous() for t in out):
         raise ValueError("compact_pages: the new tables are laid out like the old ones")
     device = _check_device("compact_pages", block_table, refs, *out, *caches)
-    scratch = refs.new_empty(8 * (R + N) + 16)   # b200_pages_scratch
+    scratch = refs.new_empty(_pages_scratch(R, N))
     _launch("b200_compact_pages", 2, device, block_table.data_ptr(), out[0].data_ptr(), refs.data_ptr(), out[1].data_ptr(), R, W, N, page or 1, tensors, len(caches),
             scratch.data_ptr())
     return out
