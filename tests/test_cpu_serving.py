@@ -246,3 +246,23 @@ def test_rows_outside_32_bits_stay_outside():
 def test_pages_scratch_holds_both_layouts(R, N):
     """Room: moves (4 words) and plans (4) of the rows, three lists of pages, a count. Compaction: moves (4 words) and three lists of pages, a count."""
     assert ops._pages_scratch(R, N) >= max(8 * R + 3 * N + 1, 7 * N + 1)
+
+
+@pytest.mark.parametrize("tokens", [1, 3])
+def test_pool_prefix_table_outlives_the_first_row(tokens):
+    """The row that was forked ends (or is cut back), rows of other prompts that are no longer than the shared keys stand in front: the pages of the
+    shared keys come from the first row that reaches beyond them."""
+    shared, page = 20, 8
+    c = prefix_batch(5, tokens, 4, 2, 64, page, shared, 12, dtype=torch.float32, lens=[30, 25, 0, 26, 30])
+    want, _ = ref.shared_prefix_attention_ref(**c)
+    pool = PagePool(1, c["k_cache"].shape[0] - 1, 5, 32, 2, 64, torch.float32, page_size=page, device="cpu")
+    pool.block_table.copy_(c["block_table"]), pool.kv_lens.copy_(c["kv_lens"])
+    pool.block_table[0], pool.kv_lens[0] = -1, 0
+    pool.block_table[1, :3], pool.kv_lens[1] = c["block_table"][4, 1:].flip(0), shared + tokens - 2     # another text
+    c["block_table"], c["kv_lens"] = pool.block_table, pool.kv_lens
+    first = pool.prefix_table(shared, tokens)
+    assert first.dtype == torch.int32 and first.shape == (4,) and first.is_contiguous()
+    got, _ = ref.shared_prefix_attention_ref(**c, prefix_table=first)
+    torch.testing.assert_close(got[2 * tokens:], want[2 * tokens:], rtol=0, atol=0)
+    pool.kv_lens.zero_()
+    assert pool.prefix_table(shared, tokens).shape == (4,)      # nobody reads it then

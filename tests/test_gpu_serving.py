@@ -728,3 +728,32 @@ def test_rows_that_32_bits_do_not_hold_are_skipped():
     _same(got, state)
     ops.trim_pages(*got, 4, None, far)
     _same(got, ref.trim_pages_ref(*state, 4, None, [0]))
+
+
+def test_samples_go_on_when_the_first_row_has_ended():
+    """Row 0, whose prompt the others share, ends and the pages are compacted: in a captured step too, the others attend as they would alone."""
+    from triton_distributed_b200 import ops, ref
+    from triton_distributed_b200.models import PagePool
+    torch.manual_seed(4)
+    pool = PagePool(1, 40, 20, 256, 2, 128, page_size=16)
+    n = torch.zeros(20, dtype=torch.int32, device="cuda")
+    n[0] = 150
+    pool.reserve(n)
+    pool.k_cache.normal_(), pool.v_cache.normal_()
+    pool.advance(n)
+    pool.fork([0] * 19, list(range(1, 20)))
+    pool.reserve(1), pool.advance(1)
+    q = torch.randn(20, 16, 128, device="cuda", dtype=torch.bfloat16)
+    call = lambda: ops.shared_prefix_attention(q, *pool.layer(0), pool.kv_lens, pool.block_table, 150, 128 ** -0.5, prefix_table=pool.prefix_table(150))  # noqa: E731
+    before = call()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        out = call()
+    for gone in ([0], [1, 2]):
+        pool.free(gone)
+        pool.compact()
+        g.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out[3:], before[3:]) and bool((out[gone] == 0).all())
+    want, _ = ref.shared_prefix_attention_ref(q, *pool.layer(0), pool.kv_lens, pool.block_table, 0, 128 ** -0.5)
+    torch.testing.assert_close(out.double(), want, rtol=2 ** -7, atol=2 ** -6)   # rounded weights and output, values below 5.5

@@ -204,6 +204,12 @@ class PagePool:
         blk = torch.where((blk >= 0) & (at < self.block_table.shape[1]) & alone, blk, self.num_blocks)
         return (blk * self.page_size + pos % self.page_size).reshape(-1)
 
+    def prefix_table(self, shared: int, tokens: int = 1) -> torch.Tensor:
+        """Pages of the first row that attends beyond its first `shared` keys with all its last `tokens` tokens -> int32 [max_blocks], for
+        ``ops.shared_prefix_attention``: row 0, its default, may have ended. Of this step: pages change with ``trim``, ``free`` and ``compact``."""
+        row = (self.kv_lens - tokens + 1 >= shared).to(torch.int32).argmax()
+        return self.block_table.index_select(0, row.view(1))[0]
+
     def advance(self, count) -> None:
         """The next `count` tokens (a number, or int32 [batch]) of every row have been written."""
         self.kv_lens += count

@@ -1071,7 +1071,7 @@ def shared_prefix_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: tor
     q [B * tokens, Hq, D], 16-bit, rows may be strided; caches [num_blocks, page, Hkv, D] in the type of q, D 64 or 128; kv_lens int32 [B] with the
     new tokens; block_table int32 [B, max_blocks]. Query token t of sequence b attends keys j < kv_lens[b] - tokens + t + 1; a row
     without any gives zeros. What is not a page of the cache, or lies behind the table, counts as keys and values of zero. Keys j < ``shared`` are read through ``prefix_table`` (int32 [>= ceil(shared / page)], default: the first
-    row of the block table, which has to hold them then) for every sequence that reaches beyond them with all its tokens; shorter sequences (also
+    row of the block table, which has to hold them then, also when its own sequence has ended: ``PagePool.prefix_table`` names a row that does) for every sequence that reaches beyond them with all its tokens; shorter sequences (also
     kv_lens 0) are attended over their own table alone. ``shared`` need not be a multiple of the page. ``max_kv_len``: an upper bound on kv_lens for the choice
     of splits (default: what the table can hold). ``variant``: which kernel reads the shared keys, "warp" (warp-level products, any page) or "tc" (tcgen05 tiles; pages
     of a multiple of 8); None picks by the rows per KV head. Returns [B * tokens, Hq, D] (and the natural-log LSE fp32 [B * tokens, Hq])."""
