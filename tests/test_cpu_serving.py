@@ -266,3 +266,21 @@ def test_pool_prefix_table_outlives_the_first_row(tokens):
     torch.testing.assert_close(got[2 * tokens:], want[2 * tokens:], rtol=0, atol=0)
     pool.kv_lens.zero_()
     assert pool.prefix_table(shared, tokens).shape == (4,)      # nobody reads it then
+
+
+@pytest.mark.parametrize("B,T,heads,kv,page,dim", [(1, 1, 8, 8, 64, 128), (2, 1, 32, 8, 16, 128), (16, 1, 64, 8, 64, 128), (24, 5, 40, 8, 16, 128), (48, 3, 14, 2, 32, 64),
+                                                   (64, 1, 64, 8, 64, 128), (256, 1, 8, 1, 128, 128), (9, 4, 160, 1, 64, 64)])
+@pytest.mark.parametrize("variant", [None, "warp", "tc"])
+def test_ranges_of_shared_keys_lie_side_by_side(B, T, heads, kv, page, dim, variant):
+    """The ranges as the launch forms them (chunks of whole slices or steps) cover the shared keys once, and none of the tensor-core kernel's is without
+    a step of its own where there are as many steps as ranges."""
+    if variant == "tc" and heads // kv > 128:
+        pytest.skip("refused: a group that no tile holds")
+    for shared in (1, 63, 64, 65, 127, 128, 129, 1000, 2048, 7001, 16384, 100003):
+        for own in (1, 300, 5000):
+            tc, ranges, _ = ops.choose_prefix_splits(B, T, heads, kv, -(-shared // 128) * 128, max(64, -(-own // 64) * 64), page, dim=dim, variant=variant)
+            unit = 128 if tc else 64
+            chunk = -(-(-(-shared // ranges)) // unit) * unit
+            edges = [(min(shared, i * chunk), min(shared, (i + 1) * chunk)) for i in range(ranges)]
+            assert edges[0][0] == 0 and edges[-1][1] == shared and all(a[1] == b[0] for a, b in zip(edges, edges[1:]))
+            assert 1 <= ranges <= min(64, -(-shared // 128))

@@ -757,3 +757,27 @@ def test_samples_go_on_when_the_first_row_has_ended():
         assert torch.equal(out[3:], before[3:]) and bool((out[gone] == 0).all())
     want, _ = ref.shared_prefix_attention_ref(q, *pool.layer(0), pool.kv_lens, pool.block_table, 0, 128 ** -0.5)
     torch.testing.assert_close(out.double(), want, rtol=2 ** -7, atol=2 ** -6)   # rounded weights and output, values below 5.5
+
+
+@pytest.mark.parametrize("variant", ["warp", "tc"])
+@pytest.mark.parametrize("B,T,Hq,Hkv,D,page", [(1, 1, 8, 8, 128, 16), (7, 1, 16, 2, 64, 64), (30, 4, 20, 4, 128, 24), (150, 1, 8, 1, 64, 128)])
+def test_every_key_counts_once(B, T, Hq, Hkv, D, page, variant):
+    """Queries of zero give every key a weight of one, and the log-sum-exp is the logarithm of the number of visible keys, whatever the ranges. Fewer than
+    42000 keys, so one key more or less is 2.3e-5 and more; sums of ones are exact, and what is left is the rounding of logarithms below 11 (log2
+    below 16) of a range and of their merge, below ten halves of a unit of 2^-20: 5e-6."""
+    from triton_distributed_b200 import ops
+    k = torch.randn(64, page, Hkv, D, device="cuda").bfloat16()
+    v = torch.ones_like(k)
+    q = torch.zeros(B * T, Hq, D, device="cuda", dtype=torch.bfloat16)
+    for shared in (1, 128, 129, 1000, 5003, 40000):
+        for own in (1, 77, 1900):
+            g = torch.Generator().manual_seed(shared + own)
+            lens = (shared + torch.randint(T, T + own, (B,), generator=g)).int().cuda()
+            if B > 1:
+                lens[B // 2] = min(shared, 50)                  # ends inside the shared keys
+            table = torch.randint(0, 64, (B, -(-(shared + own + T) // page)), generator=g).int().cuda()
+            out, lse = ops.shared_prefix_attention(q, k, v, lens, table, shared, 1.0, tokens=T, return_lse=True, variant=variant)
+            seen = (lens.double()[:, None] - T + 1 + torch.arange(T, device="cuda")).clamp_min(0).reshape(-1, 1)
+            assert bool(((lse.double() - seen.log()).abs() < 1e-5).logical_or((seen == 0) & (lse == float("-inf"))).all()), (shared, own)
+            assert torch.equal(out, (seen > 0).to(out.dtype)[..., None].expand_as(out)), (shared, own)
+    ops.check_pipeline_status()
