@@ -781,3 +781,33 @@ def test_every_key_counts_once(B, T, Hq, Hkv, D, page, variant):
             assert bool(((lse.double() - seen.log()).abs() < 1e-5).logical_or((seen == 0) & (lse == float("-inf"))).all()), (shared, own)
             assert torch.equal(out, (seen > 0).to(out.dtype)[..., None].expand_as(out)), (shared, own)
     ops.check_pipeline_status()
+
+
+@pytest.mark.parametrize("sampled", [True, False])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_drafted_tokens_follow_the_target_at_every_place(sampled, dtype):
+    """Sampled drafts, and ones that were looked up: the token at each place, among the sequences that got as far, is distributed as the target's row says. A
+    frequency among n sequences is off by more than 5 * sqrt(0.25 / n) once in 1.7e6 times; uniform numbers in steps of 2^-24 add less than 1e-6. The
+    probabilities are multiples of 1 / 128, which 16 bits hold, so that the rows' sums are exactly one."""
+    from triton_distributed_b200 import ops
+    B, K, V = 400000, 3, 6
+    g = torch.Generator(device="cuda").manual_seed(11)
+    def rows(n):
+        parts = (torch.softmax(torch.randn(n, V, device="cuda", generator=g) * 1.2, -1) * 120).floor() + 1
+        parts[:, 0] += 128 - parts.sum(-1)
+        return (parts / 128).to(dtype)
+
+    p, q = rows(K + 1), rows(K)
+    if sampled:
+        drafts = torch.stack([torch.multinomial(q[i].float(), B, replacement=True, generator=g) for i in range(K)], 1)
+    else:
+        drafts = p[:K].float().argmax(-1).expand(B, K).contiguous()
+    u = torch.rand(B, K + 1, device="cuda", generator=g)
+    accepted, tokens = ops.verify_drafts(drafts, p.expand(B, K + 1, V), u, q.expand(B, K, V) if sampled else None)
+    for place in range(K + 1):
+        got = tokens[accepted >= place, place]
+        n = got.numel()
+        assert n > 2000
+        want = p[place].double()
+        freq = torch.bincount(got, minlength=V).double() / n
+        assert float((freq - want).abs().max()) < 5 * (0.25 / n) ** 0.5 + 1e-6, (place, freq, want)
