@@ -176,12 +176,14 @@ __global__ void __launch_bounds__(kPlanThreads) reserve_plan_kernel(const Reserv
   auto entry = [&](int r, int w) -> int& { return p.table[static_cast<size_t>(r) * p.W + w]; };
   auto count_of = [&](int r) { return p.counts ? max(0, p.counts[r]) : p.count; };
   // ---- shared pages that are written into ----
+  bool gap = false;
   for (int r = r0; r < r1; ++r) {
     const int c = count_of(r), len = max(0, p.lens[r]);
     int copy = -1;
-    if (c > 0 && len % p.page != 0 && len / p.page < p.W) {
-      const int pg = entry(r, len / p.page);
-      if (pg >= 0 && pg < p.N && p.refs[pg] > 1) copy = pg;
+    if (c > 0 && len > 0 && (len - 1) / p.page < p.W) {
+      const int pg = entry(r, (len - 1) / p.page);   // of the last token
+      gap |= pg < 0;
+      if (len % p.page != 0 && pg >= 0 && pg < p.N && p.refs[pg] > 1) copy = pg;
     }
     p.rows[r].copy = copy;
     if (copy >= 0) { p.asks[copy] = 0; p.lowest[copy] = 0x7fffffff; }
@@ -200,7 +202,6 @@ __global__ void __launch_bounds__(kPlanThreads) reserve_plan_kernel(const Reserv
     if (plan.copy >= 0 && __ldcg(p.asks + plan.copy) == p.refs[plan.copy] && __ldcg(p.lowest + plan.copy) == r) plan.copy = -1;
     const long long need = c > 0 ? (static_cast<long long>(len) + c + p.page - 1) / p.page : 0;
     if (need > p.W) atomicExch(&s_too_long, 1);
-    else if (need > 0 && len > 0 && entry(r, pages_of(len, p.page) - 1) < 0) atomicExch(&s_gap, 1);
     plan.need = static_cast<int>(min(need, static_cast<long long>(p.W)));
     plan.held = min(plan.need, pages_of(len, p.page));
     while (plan.held < plan.need && entry(r, plan.held) >= 0) ++plan.held;   // room from an earlier call
@@ -208,6 +209,7 @@ __global__ void __launch_bounds__(kPlanThreads) reserve_plan_kernel(const Reserv
     sum += (plan.copy >= 0) + plan.need - plan.held;
     p.rows[r] = plan;
   }
+  if (gap) atomicExch(&s_gap, 1);
   const int before = block_scan(sum, warp_sums, total) - sum;
   // ---- the lowest free pages, as many as are asked for ----
   int found = 0;
