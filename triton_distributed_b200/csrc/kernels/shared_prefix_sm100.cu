@@ -14,8 +14,9 @@
 // Tensor memory: S of tile t at columns 128 t, O of tile t at 256 + 128 t. P is written over S as 16-bit pairs and is the A operand of
 // the second product; V is read in place as an MN-major B operand.
 // The softmax of a step does not wait for its maximum: the weights are taken against the reference of the steps before (at the first step: the maximum
-// of its first 32 keys), and only if one of a warp's scores lies above it by more than 8 the warp raises its rows' references to their maxima, rescales
-// their output and takes the step's weights anew from the scores, which are still there because the weights stay in registers until then. The maximum
+// of its first 32 keys), and only if one of a warp's scores lies above it by more than 8 (a factor of 256; published as conditional rescaling,
+// FlashAttention-4, Zadouri et al. 2026) the warp raises its rows' references to their maxima, rescales their output and takes the step's weights
+// anew from the scores, which are still there because the weights stay in registers until then. The maximum
 // of the first keys mostly stands, so this is rare, and the chain of a step is one pass over the scores instead of two (two passes at the first step
 // only, for the maximum of all its keys: 18.0 instead of 17.1 us for 16 rows of 64 / 8 heads over 2048 keys). Weights above one are rounded like those
 // below (relative to themselves); what is lost is that a row's largest weight was held exactly: error against 64 bits 2.3e-3 of the norm both ways.

@@ -100,7 +100,8 @@ template <typename T> constexpr int kGroupBlocks = 32 * kGroupRows<T, 1>;       
 
 // The sum of the weights of blocks [k0, k1), by a warp; `sums` [kVerifySlots][32] receives each lane's sums of `per_slot` groups of kGroupBlocks. (Adding
 // them up over the lanes, ten shuffles and five dependent additions in 64 bits a group, took 3 us of 64 sequences' 24.) kQ: 0 without draft
-// probabilities, 1 with them aligned like the target's, 2 otherwise.
+// probabilities, 1 with them aligned like the target's, 2 otherwise: the draft's values are then loaded one by one (64 sequences with draft probabilities,
+// 50257 tokens for 50256: 12.6 us for 10.8 in 32 bits, 9.7 for 7.6 in 16).
 // Whole blocks in groups of loads, each issued before the values of the group in front are used; loads behind the end are of the last block, without a
 // weight, so that no branch stands between loads. A block that the row's ends cut is read token by token.
 // The first form looked at every value for what is no probability and kept the last token with a weight: about thirty instructions a
